@@ -107,7 +107,9 @@ typedef struct {
 /* Declared shape and element type of a graph input (TensorInfo, oxionnx-core src/graph.rs:862).
  * dtype 0 (f32 lanes) is the reference's dtype-erased convention; U8 / I8 declare a quantised
  * input whose feeds arrive as typed 8-bit lanes and whose saturation is exact per type
- * (SatRange::for_dtype, oxionnx-ops src/registry/quant_ops/mod.rs:216-222). */
+ * (SatRange::for_dtype, oxionnx-ops src/registry/quant_ops/mod.rs:216-222).  F16, BF16 and I32 inputs are stored, fed (as
+ * `typed` lanes) and bound in that type; the decoder operators (MatMulNBits, OxiPagedCacheAppend, OxiPagedAttention) read
+ * them so, every other operator reads an f32 copy. */
 typedef struct {
   const char* name;
   const uint64_t* shape;
@@ -299,6 +301,21 @@ float oxb200_last_run_ms(const oxb200_ctx* ctx);
  *   clear_bindings      forgets every binding; later runs upload and download as before. */
 int oxb200_bind_input_device(oxb200_ctx* ctx, const char* name, const void* device_ptr, int32_t dtype, uint64_t len);
 int oxb200_bind_output_device(oxb200_ctx* ctx, const char* name, void* device_ptr, uint64_t cap);
+/* bind_output_device in the output's own element type (`dtype`, the type the graph gives it: f16 and bf16 outputs of the
+ * decoder operators, f32 otherwise): the lanes go to `device_ptr` alone, and where nobody fetches them no f32 copy is made.
+ * 16-byte aligned buffers that share no memory with another bound buffer are written in place.  While an output is bound so,
+ * output_device_ptr and fetch_value refuse it.
+ *   run_enqueue         run_bound without its fence, on `cuda_stream` (a cudaStream_t of the context's device, NULL: the
+ *                       default stream): every input must be bound, nothing is fetched, and the call returns when the
+ *                       launches are in the stream.  Bound buffers follow that stream's order like any kernel's operands.
+ *                       Runs of one session follow one another whatever their streams; a stream that is being captured
+ *                       takes the launches into its graph with the addresses bound now, and its replays are then the
+ *                       caller's to order against the session's other runs.  The caller's current device is kept.
+ *   run_wait            waits for the enqueued runs and reports what their kernels found wrong (a page table entry outside
+ *                       the cache, ...), as every call that fences does. */
+int oxb200_bind_output_device_typed(oxb200_ctx* ctx, const char* name, void* device_ptr, int32_t dtype, uint64_t cap);
+int oxb200_run_enqueue(oxb200_ctx* ctx, void* cuda_stream);
+int oxb200_run_wait(oxb200_ctx* ctx);
 int oxb200_output_device_ptr(oxb200_ctx* ctx, const char* name, void** device_ptr, uint64_t* len);
 int oxb200_run_bound(oxb200_ctx* ctx, const oxb200_operand* feeds, uint32_t n_feeds, oxb200_result* fetches, uint32_t n_fetches);
 int oxb200_clear_bindings(oxb200_ctx* ctx);

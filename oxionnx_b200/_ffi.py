@@ -14,6 +14,34 @@ MAX_RANK = 8
 DT_F32, DT_U8, DT_I8, DT_I32, DT_F16, DT_BF16 = 0, 1, 2, 3, 5, 6
 # numpy element types that cross the boundary as typed lanes
 TYPED = {np.dtype(np.uint8): DT_U8, np.dtype(np.int8): DT_I8}
+# element types by name: what inputs may be declared and buffers bound as
+NAMED = {"float32": DT_F32, "uint8": DT_U8, "int8": DT_I8, "int32": DT_I32, "float16": DT_F16, "bfloat16": DT_BF16}
+
+
+def dtype_code(t):
+    """OXB200_DT_* of a type's name, or of a numpy type (of those only the 8-bit ones are types of the boundary: the others
+    are fed as f32 lanes)."""
+    if isinstance(t, str) and t in NAMED:
+        return NAMED[t]
+    return TYPED.get(np.dtype(t), DT_F32)
+
+
+def lanes_of(a, code):
+    """The lanes of a feed for an input declared `code`, as the library reads them: f32 or typed as they are, rounded to 16
+    bits (bf16 as its bit patterns) or taken as int32 where the input was declared so."""
+    if code == DT_F16:
+        return np.ascontiguousarray(a, dtype=np.float16)
+    if code == DT_BF16:
+        f = np.ascontiguousarray(a, dtype=np.float32)
+        bits = f.view(np.uint32)
+        rounded = ((bits + 0x7FFF + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
+        return np.where(np.isnan(f), np.uint16(0x7FC0), rounded).reshape(f.shape)
+    if code == DT_I32:
+        return np.ascontiguousarray(a).astype(np.int32)
+    typed = isinstance(a, np.ndarray) and a.dtype in TYPED
+    return np.ascontiguousarray(a if typed else np.asarray(a, dtype=np.float32))
+
+
 OK_HOST, OK_DEVICE, DECLINED, FAILED, VERIFY_MISMATCH = 0, 1, 2, 3, 4
 PLACE_HOST, PLACE_DEVICE = 0, 1
 STATUS_NAMES = {0: "OK_HOST", 1: "OK_DEVICE", 2: "DECLINED", 3: "FAILED", 4: "VERIFY_MISMATCH"}
@@ -122,6 +150,9 @@ SYMBOLS = {
     "oxb200_bind_output_device": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_uint64]),
     "oxb200_output_device_ptr": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, _P(ctypes.c_void_p), _P(ctypes.c_uint64)]),
     "oxb200_run_bound": (ctypes.c_int, [ctypes.c_void_p, _P(Operand), ctypes.c_uint32, _P(Result), ctypes.c_uint32]),
+    "oxb200_bind_output_device_typed": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint64]),
+    "oxb200_run_enqueue": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "oxb200_run_wait": (ctypes.c_int, [ctypes.c_void_p]),
     "oxb200_clear_bindings": (ctypes.c_int, [ctypes.c_void_p]),
     "oxb200_upload_feeds": (ctypes.c_int, [ctypes.c_void_p, _P(Operand), ctypes.c_uint32]),
     "oxb200_run_resident": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_uint32, _P(ctypes.c_float)]),
@@ -237,18 +268,18 @@ def packed_node(node):
     return have
 
 
-def pack_operand(op, name, array, keep, resident=None):
+def pack_operand(op, name, array, keep, resident=None, dtype=DT_F32):
     op.name = name.encode()
     if resident is not None:
         op.resident = resident
         return
     if array is None:
         return
-    if isinstance(array, np.ndarray) and array.dtype in TYPED:
-        # 8-bit lanes of a graph input that was declared with that type
+    if dtype in (DT_F16, DT_BF16, DT_I32) or (isinstance(array, np.ndarray) and array.dtype in TYPED):
+        # lanes in the type that a graph input was declared with
         a = keep.add(np.ascontiguousarray(array))
         op.typed = a.ctypes.data_as(ctypes.c_void_p)
-        op.dtype = TYPED[a.dtype]
+        op.dtype = TYPED.get(a.dtype, dtype) if dtype == DT_F32 else dtype
         op.len = a.size
         op.shape = keep.add((ctypes.c_uint64 * max(a.ndim, 1))(*a.shape))
         op.rank = a.ndim

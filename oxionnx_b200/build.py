@@ -24,11 +24,14 @@ KERNEL = [f for f in COMMON if f != "--fmad=false"]
 OBJECTS = {
     "kernels_glue": ("kernels_glue.cu", COMMON),
     **{name: (name + ".cu", KERNEL) for name in ("kernels_simt", "kernels_umma", "umma_i8", "umma_tf32", "umma_f16", "umma_small_i8", "umma_small_float",
-                                                  "umma_probe", "umma_chain", "umma_attention")},
+                                                  "umma_probe", "umma_chain", "umma_attention", "paged_append", "paged_attention", "linear4")},
     **{f"umma_i8_{tile}": ("umma_i8_tile.cu", KERNEL + [f"-DOXB_TILE={bn}", f"-DOXB_PAIR={pair}"])
        for tile, bn, pair in (("32", 32, "false"), ("64", 64, "false"), ("128", 128, "false"), ("256", 256, "false"), ("pair", 256, "true"))},
     **{name: (name + ".cpp", COMMON) for name in ("runtime", "planner", "abi", "onnx_model", "model_abi")},
 }
+# headers of the decoder operators, which nothing but these objects includes
+DECODER_HEADERS = ["decoder.hpp", "decoder_device.cuh"]
+DECODER_OBJECTS = ("planner", "paged_append", "paged_attention", "linear4")
 HEADERS = ["common.hpp", "kernels.hpp", "runtime.hpp", "umma_kernel.cuh", "umma_epilogue8.cuh", "umma_launch.cuh", "umma_small.cuh", "pdl.cuh", "umma_chain.cuh", "model.hpp", "abi_internal.hpp", os.path.join("..", "..", "include", "oxb200.h")]
 
 
@@ -49,6 +52,7 @@ def _stale(target, deps):
 def build(force=False, verbose=False):
     os.makedirs(OBJ_DIR, exist_ok=True)
     headers = [os.path.join(CSRC, h) for h in HEADERS]
+    decoder_headers = [os.path.join(CSRC, h) for h in DECODER_HEADERS]
     nvcc = _nvcc()
     jobs = []
     objs = []
@@ -56,7 +60,7 @@ def build(force=False, verbose=False):
         path = os.path.join(CSRC, src)
         obj = os.path.join(OBJ_DIR, name + ".o")
         objs.append(obj)
-        if force or _stale(obj, [path] + headers):
+        if force or _stale(obj, [path] + headers + (decoder_headers if name in DECODER_OBJECTS else [])):
             cmd = [nvcc] + ARCH + flags + ["-x", "cu", "-c", path, "-o", obj]
             if verbose:
                 cmd.insert(1, "-Xptxas=-v")

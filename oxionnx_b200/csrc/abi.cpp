@@ -594,6 +594,9 @@ int oxb200_session_plan(oxb200_ctx* ctx, const oxb200_node* nodes, uint32_t n_no
         case OXB200_DT_F32: return DT::F32;
         case OXB200_DT_U8: return DT::U8;
         case OXB200_DT_I8: return DT::I8;
+        case OXB200_DT_I32: return DT::I32;
+        case OXB200_DT_F16: return DT::F16;
+        case OXB200_DT_BF16: return DT::BF16;
         default: raise(OXB200_DECLINED, "graph input '%s': element type %d is not taken at the boundary", name, (int)d);
       }
     };
@@ -608,6 +611,26 @@ int oxb200_session_plan(oxb200_ctx* ctx, const oxb200_node* nodes, uint32_t n_no
     return (int)OXB200_OK_DEVICE;
   });
 }
+
+// Element types of bound buffers.
+static DT boundary_dt(const char* call, int32_t dtype) {
+  switch (dtype) {
+    case OXB200_DT_F32: return DT::F32;
+    case OXB200_DT_U8: return DT::U8;
+    case OXB200_DT_I8: return DT::I8;
+    case OXB200_DT_I32: return DT::I32;
+    case OXB200_DT_F16: return DT::F16;
+    case OXB200_DT_BF16: return DT::BF16;
+    default: raise(OXB200_FAILED, "%s: element type %d is not taken at the boundary", call, (int)dtype);
+  }
+}
+
+// A call that works on a caller's stream leaves the caller's current device as it was.
+struct CallersDevice {
+  int device = -1;
+  CallersDevice() { OXB_CUDA(cudaGetDevice(&device)); }
+  ~CallersDevice() { cudaSetDevice(device); }
+};
 
 static Session& planned(oxb200_ctx* ctx) {
   if (!ctx->impl.session) raise(OXB200_FAILED, "no session has been planned on this context");
@@ -674,14 +697,7 @@ int oxb200_bind_input_device(oxb200_ctx* ctx, const char* name, const void* devi
   return guarded(ctx, [&]() {
     std::lock_guard<std::mutex> lock(ctx->impl.mu);
     ctx->impl.make_current();
-    DT dt;
-    switch (dtype) {
-      case OXB200_DT_F32: dt = DT::F32; break;
-      case OXB200_DT_U8: dt = DT::U8; break;
-      case OXB200_DT_I8: dt = DT::I8; break;
-      default: raise(OXB200_FAILED, "bind_input_device: element type %d is not taken at the boundary", (int)dtype);
-    }
-    planned(ctx).bind_input_device(name, device_ptr, dt, len);
+    planned(ctx).bind_input_device(name, device_ptr, boundary_dt("bind_input_device", dtype), len);
     return (int)OXB200_OK_HOST;
   });
 }
@@ -693,6 +709,38 @@ int oxb200_bind_output_device(oxb200_ctx* ctx, const char* name, void* device_pt
     ctx->impl.make_current();
     planned(ctx).bind_output_device(name, device_ptr, cap);
     return (int)OXB200_OK_HOST;
+  });
+}
+
+int oxb200_bind_output_device_typed(oxb200_ctx* ctx, const char* name, void* device_ptr, int32_t dtype, uint64_t cap) {
+  if (!ctx || !name) return fail_with(ctx, OXB200_FAILED, "bind_output_device: NULL argument");
+  return guarded(ctx, [&]() {
+    std::lock_guard<std::mutex> lock(ctx->impl.mu);
+    ctx->impl.make_current();
+    planned(ctx).bind_output_device(name, device_ptr, cap, true, boundary_dt("bind_output_device", dtype));
+    return (int)OXB200_OK_HOST;
+  });
+}
+
+int oxb200_run_enqueue(oxb200_ctx* ctx, void* cuda_stream) {
+  if (!ctx) return fail_with(ctx, OXB200_FAILED, "run_enqueue: ctx is NULL");
+  return guarded(ctx, [&]() {
+    std::lock_guard<std::mutex> lock(ctx->impl.mu);
+    CallersDevice device;
+    ctx->impl.make_current();
+    planned(ctx).enqueue((cudaStream_t)cuda_stream);
+    return (int)OXB200_OK_DEVICE;
+  });
+}
+
+int oxb200_run_wait(oxb200_ctx* ctx) {
+  if (!ctx) return fail_with(ctx, OXB200_FAILED, "run_wait: ctx is NULL");
+  return guarded(ctx, [&]() {
+    std::lock_guard<std::mutex> lock(ctx->impl.mu);
+    CallersDevice device;
+    ctx->impl.make_current();
+    planned(ctx).run_wait();
+    return (int)OXB200_OK_DEVICE;
   });
 }
 

@@ -36,6 +36,8 @@ __device__ __forceinline__ float load_as_f32(const void* p, DT dt, int64_t i) {
     case DT::I8: return (float)((const int8_t*)p)[i];
     case DT::I32: return __int2float_rn(((const int32_t*)p)[i]);
     case DT::I16: return (float)((const int16_t*)p)[i];
+    case DT::F16: return __half2float(((const __half*)p)[i]);
+    case DT::BF16: return __bfloat162float(((const __nv_bfloat16*)p)[i]);
   }
   return 0.f;
 }

@@ -245,7 +245,7 @@ int oxb200_session_plan_model(oxb200_ctx* ctx, oxb200_model* m, const oxb200_val
       for (int64_t d : sh)
         if (d < 0) raise(OXB200_FAILED, "session_plan_model: input '%s' has a symbolic dimension; pass its concrete shape", vi.name.c_str());
       DT dt;
-      if (!onnx_dtype_to_dt(vi.onnx_dtype, &dt) || !(dt == DT::F32 || dt == DT::U8 || dt == DT::I8))
+      if (!onnx_dtype_to_dt(vi.onnx_dtype, &dt) || dt == DT::I16)
         raise(OXB200_DECLINED, "session_plan_model: input '%s' has ONNX element type %d, which the boundary does not take", vi.name.c_str(), (int)vi.onnx_dtype);
       sess->declare_input_type(vi.name, dt);
       in.push_back({vi.name, sh});

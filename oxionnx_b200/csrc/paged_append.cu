@@ -1,0 +1,164 @@
+// New tokens into a paged cache: queries and keys are rotated by their positions, keys and values go to their rows of the
+// pages.  Memory bound: every lane is read once and written once, and a pair (a, b) of lanes at position p becomes
+// (a cos - b sin, b cos + a sin) with the row p of cos and sin, in f32, rounded once.
+#include "decoder_device.cuh"
+
+namespace oxb {
+namespace k {
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+
+enum class Turn { None, Halves, Pairs, Lanes };  // pairs a half apart / side by side, in 16-byte steps; lane by lane
+
+template <typename T>
+struct alignas(16) Eight {
+  T v[8];
+};
+
+template <typename TI>
+__device__ __forceinline__ void load8(const TI* p, float* x) {
+  if constexpr (sizeof(TI) == 4) {
+    const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    const Eight<TI> r = *(const Eight<TI>*)p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32(r.v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* x) {
+  Eight<T> r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = from_f32<T>(x[i]);
+  *(Eight<T>*)p = r;
+}
+
+// One block serves one token (or a part of its heads).  An item is the 16 bytes of one head that a thread takes, or with
+// Turn::Halves the two times 16 bytes whose lanes turn together.
+template <typename TI, typename T, Turn TURN>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(PagedAppend a, int parts, int items_rotated, int items_plain) {
+  pdl_enter();
+  const int64_t token = blockIdx.x / parts;
+  const int item = (int)(blockIdx.x % parts) * kAppendThreads + threadIdx.x;
+  const int turned = (a.heads + a.kv_heads) * items_rotated;
+  int head, at;  // heads of q, then of k, then of v
+  if (item < turned) head = item / items_rotated, at = item % items_rotated;
+  else head = a.heads + a.kv_heads + (item - turned) / items_plain, at = (item - turned) % items_plain;
+  const bool mine = item < turned + a.kv_heads * items_plain;
+  const bool is_q = head < a.heads, is_v = head >= a.heads + a.kv_heads;
+  const int h = is_q ? head : (head - a.heads) % a.kv_heads;
+  const TI* src = (is_q ? (const TI*)a.q + token * a.q_stride : is_v ? (const TI*)a.v + token * a.v_stride : (const TI*)a.k + token * a.k_stride) + (int64_t)h * a.size;
+
+  // where the item's lanes lie in the head, and whether they turn
+  int lane = at * 8;
+  bool turns = TURN != Turn::None && !is_v, two = false;
+  if (TURN == Turn::Halves && turns) {
+    two = at < a.half / 8;
+    if (!two) lane = 2 * a.half + (at - a.half / 8) * 8, turns = false;
+  } else if (turns) {
+    turns = lane < 2 * a.half;
+  }
+  float x[8], y[8];
+  if (mine) {  // does not wait for the search below
+    load8(src + lane, x);
+    if (two) load8(src + lane + a.half, y);
+  }
+
+  // the token's sequence: how many of the row bounds behind the first lie at or before it, a warp's width at a time
+  int b = 0;
+  for (int base = 0; base < a.t.sequences; base += 32) {
+    const int i = base + (threadIdx.x & 31);
+    b += __popc(__ballot_sync(0xffffffffu, i < a.t.sequences && a.t.cu_query[i + 1] <= token));
+  }
+  int64_t position = -1, slot = -1;
+  int wrong = 0;
+  if (b < a.t.sequences) {
+    bool bad;
+    const Sequence q = sequence_of(a.t, b, &bad);
+    if (bad || token < q.first || token >= q.first + q.rows) {
+      wrong = kErrLengths;
+    } else {
+      position = (int64_t)q.length - q.rows + (token - q.first);
+      if (position >= 0) {
+        const int page = a.t.page_table[(int64_t)b * a.t.max_pages + position / a.t.page];
+        if (a.cos && position >= a.positions) wrong = kErrPosition;
+        else if (page < 0 || page >= a.t.pages) wrong = kErrPage;
+        else slot = (int64_t)page * a.t.page + position % a.t.page;
+      }
+    }
+  } else if (token < a.t.cu_query[a.t.sequences]) {
+    wrong = kErrLengths;  // bounds that fall
+  }
+  if (wrong && threadIdx.x == 0) report(a.err, wrong);
+  if (!mine || (slot < 0 && !is_q)) return;
+
+  T* dst = is_q ? (T*)a.rotated + (token * a.heads + h) * a.size : (is_v ? (T*)a.value_cache : (T*)a.key_cache) + (slot * a.kv_heads + h) * a.size;
+  if (slot < 0) {  // a token of no sequence
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
+  } else if (turns) {
+    const float *cos = a.cos + position * a.half, *sin = a.sin + position * a.half;
+    if constexpr (TURN == Turn::Halves) {
+      float c[8], s[8];
+      load8(cos + lane, c);
+      load8(sin + lane, s);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = x[i], v = y[i];
+        x[i] = u * c[i] - v * s[i];
+        y[i] = v * c[i] + u * s[i];
+      }
+    } else if constexpr (TURN == Turn::Pairs) {
+      const float4 c = *(const float4*)(cos + lane / 2), s = *(const float4*)(sin + lane / 2);
+      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float u = x[2 * i], v = x[2 * i + 1];
+        x[2 * i] = u * cc[i] - v * ss[i];
+        x[2 * i + 1] = v * cc[i] + u * ss[i];
+      }
+    } else if constexpr (TURN == Turn::Lanes) {
+      for (int i = 0; i < 8; ++i) {
+        const int l = lane + i;
+        if (l >= 2 * a.half) break;
+        const bool second = a.interleaved ? l & 1 : l >= a.half;
+        const int other = a.interleaved ? l ^ 1 : second ? l - a.half : l + a.half, turn = a.interleaved ? l / 2 : second ? l - a.half : l;
+        const float w = to_f32(src[other]);
+        x[i] = second ? x[i] * cos[turn] + w * sin[turn] : x[i] * cos[turn] - w * sin[turn];
+      }
+    }
+  }
+  store8(dst + lane, x);
+  if (two) store8(dst + lane + a.half, y);
+}
+
+template <typename TI, typename T>
+void append_typed(const PagedAppend& a, cudaStream_t s) {
+  Turn turn = Turn::None;
+  if (a.cos) turn = a.interleaved ? (a.half % 4 == 0 ? Turn::Pairs : Turn::Lanes) : (a.half % 8 == 0 ? Turn::Halves : Turn::Lanes);
+  const int plain = a.size / 8, rotated = turn == Turn::Halves ? plain - a.half / 8 : plain;
+  const int parts = (int)ceil_div((int64_t)(a.heads + a.kv_heads) * rotated + (int64_t)a.kv_heads * plain, kAppendThreads);
+  const dim3 grid((unsigned)(a.t.tokens * parts));
+  auto go = [&](auto kernel) { launch(kernel, grid, dim3(kAppendThreads), 0, s, a, parts, rotated, plain); };
+  switch (turn) {
+    case Turn::None: return go(paged_append_kernel<TI, T, Turn::None>);
+    case Turn::Halves: return go(paged_append_kernel<TI, T, Turn::Halves>);
+    case Turn::Pairs: return go(paged_append_kernel<TI, T, Turn::Pairs>);
+    case Turn::Lanes: return go(paged_append_kernel<TI, T, Turn::Lanes>);
+  }
+}
+
+}  // namespace
+
+void paged_append(const PagedAppend& a, cudaStream_t s) {
+  if (a.t.tokens == 0) return;
+  const bool f32 = a.in_dt == DT::F32;
+  if (a.cache_dt == DT::F16) f32 ? append_typed<float, __half>(a, s) : append_typed<__half, __half>(a, s);
+  else f32 ? append_typed<float, __nv_bfloat16>(a, s) : append_typed<__nv_bfloat16, __nv_bfloat16>(a, s);
+}
+
+}  // namespace k
+}  // namespace oxb

@@ -16,6 +16,7 @@
 #include <limits>
 #include <memory>
 
+#include "decoder.hpp"
 #include "runtime.hpp"
 
 namespace oxb {
@@ -30,7 +31,10 @@ const char* kSupportedOps[] = {"Conv",       "Gemm",     "MatMul",  "QLinearConv
                                "Add",        "Sub",      "Mul",     "Div",         "MaxPool",       "GlobalAveragePool", "OxiInstanceNorm",
                                "Resize",     "Pad",      "Concat",  "Flatten",     "Reshape",       "Identity",          "Cast",
                                "Slice",      "Gather",   "Transpose", "Softmax",   "LayerNormalization", "LayerNorm",    "Gelu",
-                               "Erf",        "ConvAddRelu", "Silu",  "SiLU"};
+                               "Erf",        "ConvAddRelu", "Silu",  "SiLU",    "MatMulNBits", "OxiPagedCacheAppend", "OxiPagedAttention"};
+
+// Operators that take and give values in the types the graph declares (f16, bf16, i32) instead of f32 lanes.
+bool typed_op(const std::string& op) { return op == "MatMulNBits" || op == "OxiPagedCacheAppend" || op == "OxiPagedAttention"; }
 
 // ---- scalar helpers that must agree with the reference bit for bit -----------------------
 double round_ties_even(double v) { return std::nearbyint(v); }  // default rounding mode: ties to even
@@ -205,6 +209,7 @@ bool accepts_resident_slot(const std::string& op, uint32_t slot) {
   if (op == "Gemm") return slot == 0;
   if (op == "MatMul" || op == "Add" || op == "Sub" || op == "Mul" || op == "Div") return slot <= 1;
   if (op == "Concat") return true;
+  if (op == "OxiPagedCacheAppend" || op == "OxiPagedAttention") return false;  // they live in sessions, where their cache is bound
   if (op == "QuantizeLinear" || op == "DequantizeLinear" || op == "PRelu" || op == "Reshape" || op == "Resize" || op == "Pad") return slot == 0;
   return slot == 0;
 }
@@ -227,6 +232,7 @@ class Planner {
   std::set<std::string> graph_outputs_;
   std::map<std::pair<int, int>, int> layout_memo_;
   std::set<std::string> tf32_rounded_names_;
+  std::unordered_map<std::string, int> typed_index_;
   int cur_node_ = -1;
 
   // ---- value bookkeeping ----
@@ -268,6 +274,47 @@ class Planner {
     V(idx).ptr = C.resident_form(name, "raw_f32", bytes, [h](void* dst) { std::memcpy(dst, h->data.data(), h->data.size() * 4); },
                                  cacheable_const(name));
     return idx;
+  }
+
+  // ---- values in a declared type ----
+  // A value of type f16, bf16 or i32 that the graph names.  Where an operator that works on f32 lanes reads it, its name
+  // stands for an f32 copy (widen), and the typed value has a name of its own; typed operators find it in typed_index_.
+  bool reads_typed(const NodeDef& c, int slot) const {
+    return typed_op(c.op) || (slot == 0 && (c.op == "Reshape" || c.op == "Flatten" || c.op == "Identity"));
+  }
+  bool widened(const std::string& name) const {
+    auto it = consumers_.find(name);
+    if (it == consumers_.end()) return false;
+    for (const auto& use : it->second)
+      if (!reads_typed(nodes_[use.first], use.second)) return true;
+    return false;
+  }
+  int add_typed(const std::string& name, const std::vector<int64_t>& shape, DT dt) {
+    if (dt == DT::F32) return add_value(name, shape, dt, Layout::PLAIN);
+    if (S.index_.count(name)) OXB_FAIL("value '%s' is produced twice", name.c_str());
+    const int vi = add_value(widened(name) ? name + "@" + dt_name(dt) : name, shape, dt, Layout::PLAIN);
+    typed_index_[name] = vi;
+    return vi;
+  }
+  // Behind the step that writes a typed value: its f32 copy, where someone reads one.
+  void widen(const NodeDef& n, const std::string& name) {
+    auto it = typed_index_.find(name);
+    if (it == typed_index_.end() || !widened(name)) return;
+    const int xi = it->second;
+    const int yi = add_value(name, V(xi).shape, DT::F32, Layout::PLAIN);
+    const Dims4 d{std::max<int64_t>(V(xi).numel(), 0), 1, 1, 1};
+    TensorRef a{nullptr, V(xi).dt, Layout::PLAIN, d}, b{nullptr, DT::F32, Layout::PLAIN, d};
+    Step& st = add_step(n, "widen_to_f32", 2, {xi}, {yi});
+    st.work = (double)V(xi).bytes + (double)V(yi).bytes;
+    st.launch = [this, a, b, xi, yi](cudaStream_t s) {
+      k::convert(bound(a, xi), bound(b, yi), s);
+      C.counters.glue_launches++;
+      C.counters.kernel_launches++;
+    };
+  }
+  int typed_value_of(const std::string& name) {
+    auto it = typed_index_.find(name);
+    return it == typed_index_.end() ? value_of(name) : it->second;
   }
 
   const std::string& in_name(const NodeDef& n, size_t i) const {
@@ -459,6 +506,11 @@ class Planner {
   void plan_quantize(const NodeDef& n);
   void plan_dequantize(const NodeDef& n);
   void plan_dynamic_quantize(const NodeDef& n);
+  struct PagedInputs;
+  PagedInputs paged_inputs(const NodeDef& n, size_t first);
+  void plan_matmul_4bit(const NodeDef& n);
+  void plan_paged_append(const NodeDef& n);
+  void plan_paged_attention(const NodeDef& n);
   void plan_conv_family(const NodeDef& n, int ni);
   void plan_matmul_family(const NodeDef& n, int ni);
   void plan_unary(const NodeDef& n);
@@ -606,8 +658,9 @@ void Planner::run(const std::vector<std::pair<std::string, std::vector<int64_t>>
     // declared element type (TensorInfo): 8-bit inputs are stored, fed and bound as 8-bit lanes
     auto declared = S.input_types_.find(in.first);
     const DT in_dt = declared == S.input_types_.end() ? DT::F32 : declared->second;
-    if (!(in_dt == DT::F32 || in_dt == DT::U8 || in_dt == DT::I8)) OXB_DECLINE("graph input '%s': declared element type %s is not one this provider takes at the boundary", in.first.c_str(), dt_name(in_dt));
-    int vi = add_value(in.first, in.second, in_dt, Layout::PLAIN);
+    const bool typed = in_dt == DT::F16 || in_dt == DT::BF16 || in_dt == DT::I32;
+    if (!(in_dt == DT::F32 || in_dt == DT::U8 || in_dt == DT::I8 || typed)) OXB_DECLINE("graph input '%s': declared element type %s is not one this provider takes at the boundary", in.first.c_str(), dt_name(in_dt));
+    int vi = typed ? add_typed(in.first, in.second, in_dt) : add_value(in.first, in.second, in_dt, Layout::PLAIN);
     V(vi).is_graph_input = true;
     V(vi).external = true;
     auto vc = vconsts_.find(in.first);
@@ -623,6 +676,12 @@ void Planner::run(const std::vector<std::pair<std::string, std::vector<int64_t>>
     }
     S.input_staging_.push_back({in.first, vi});
   }
+  NodeDef in_node;
+  in_node.op = "(input)";
+  for (auto& in : inputs) {
+    in_node.name = in.first;
+    widen(in_node, in.first);
+  }
 
   for (size_t ni = 0; ni < nodes_.size(); ++ni) {
     if (skipped_[ni]) continue;
@@ -636,10 +695,23 @@ void Planner::run(const std::vector<std::pair<std::string, std::vector<int64_t>>
   out_node.op = "(output)";
   for (auto& o : outputs) {
     auto it = S.index_.find(o);
-    if (it == S.index_.end()) OXB_FAIL("graph output '%s' is not produced by any planned node", o.c_str());
-    int vi = it->second;
+    auto typed = typed_index_.find(o);
+    if (it == S.index_.end() && typed == typed_index_.end()) OXB_FAIL("graph output '%s' is not produced by any planned node", o.c_str());
+    int vi = typed != typed_index_.end() ? typed->second : it->second;
     V(vi).is_graph_output = true;
     out_node.name = o;
+    S.output_raw_.push_back(-1);
+    if (V(vi).dt == DT::F16 || V(vi).dt == DT::BF16) {
+      // kept in its own type for a caller that binds it so, and as f32 lanes for everybody else
+      S.output_raw_.back() = vi;
+      int root = vi;
+      while (V(root).alias_of >= 0) root = V(root).alias_of;
+      if (!V(root).external) {
+        V(root).external = true;
+        V(root).ptr = owned_buffer(std::max<size_t>(V(root).bytes, 256));
+      }
+      V(vi).ptr = V(root).ptr;
+    }
     // An output whose storage already holds the lanes in the logical order is handed out as it is, and so is a view of
     // such a value (Reshape, Flatten): the storage moves out of the arena into a persistent buffer.
     int root = vi;
@@ -665,6 +737,7 @@ void Planner::run(const std::vector<std::pair<std::string, std::vector<int64_t>>
     Dims4 d = V(vi).shape.size() == 4 ? dims_of(V(vi)) : Dims4{std::max<int64_t>(V(vi).numel(), 0), 1, 1, 1};
     TensorRef a{nullptr, V(vi).dt, effective_layout(V(vi)), d}, b{nullptr, DT::F32, Layout::PLAIN, d};
     Step& st = add_step(out_node, "convert_output", 2, {vi}, {so});
+    if (S.output_raw_.back() >= 0) st.host_copy_of = (int)S.output_raw_.size() - 1;
     st.work = (double)V(vi).bytes + (double)V(so).bytes;
     st.launch = [this, a, b, vi, so](cudaStream_t s) {
       k::convert(bound(a, vi), bound(b, so), s);
@@ -967,6 +1040,9 @@ void Planner::plan_node(int ni) {
   const NodeDef& n = nodes_[ni];
   const std::string& op = n.op;
   if (!is_supported_op(op)) OXB_DECLINE("operator '%s' (node '%s') is not claimed by this provider", op.c_str(), n.name.c_str());
+  if (op == "MatMulNBits") return plan_matmul_4bit(n);
+  if (op == "OxiPagedCacheAppend") return plan_paged_append(n);
+  if (op == "OxiPagedAttention") return plan_paged_attention(n);
   if (op == "Slice") return plan_slice(n);
   if (op == "Gather") return plan_gather(n);
   if (op == "Transpose") return plan_transpose(n);
@@ -3000,6 +3076,266 @@ void Planner::plan_gather(const NodeDef& n) {
   };
 }
 
+// ---- decoder operators ----------------------------------------------------------------------
+// MatMulNBits: rows times a matrix of 4-bit codes.  Inputs x [.., K], codes uint8 [N][groups][block_size / 2] (two codes a
+// byte, the even one low), scales [N][groups], optional zero points uint8 [N][ceil(groups / 2)] (two a byte; 8 without
+// them), no group index, optional bias [N].  y has x's type; sums are f32.
+void Planner::plan_matmul_4bit(const NodeDef& n) {
+  check_attrs(n, {"K", "N", "bits", "block_size", "accuracy_level"});
+  const char* name = n.name.c_str();
+  const int64_t K = n.attrs.i("K", 0), N = n.attrs.i("N", 0), group = n.attrs.i("block_size", 0);
+  if (n.attrs.i("bits", 4) != 4) OXB_DECLINE("MatMulNBits '%s': only 4-bit codes are claimed", name);
+  if (n.outputs.size() != 1) OXB_DECLINE("MatMulNBits '%s': one output", name);
+  if (K <= 0 || N <= 0 || K > (1 << 24) || N > (1 << 24)) OXB_DECLINE("MatMulNBits '%s': K %lld, N %lld", name, (long long)K, (long long)N);
+  if (group < 16 || group > 1024 || (group & (group - 1))) OXB_DECLINE("MatMulNBits '%s': block_size %lld is no power of two from 16 to 1024", name, (long long)group);
+  const int64_t groups = ceil_div(K, group);
+  const HostTensor *codes = const_in(n, 1), *scales = const_in(n, 2), *zeros = const_in(n, 3), *bias = const_in(n, 5);
+  if (has_in(n, 4)) OXB_DECLINE("MatMulNBits '%s': a group index is not claimed", name);
+  if (!codes || !scales || (has_in(n, 3) && !zeros) || (has_in(n, 5) && !bias)) OXB_DECLINE("MatMulNBits '%s': codes, scales, zero points and bias must be initializers", name);
+  if ((int64_t)codes->data.size() != N * groups * (group / 2)) OXB_DECLINE("MatMulNBits '%s': %zu bytes of codes, %lld expected", name, codes->data.size(), (long long)(N * groups * (group / 2)));
+  if ((int64_t)scales->data.size() != N * groups) OXB_DECLINE("MatMulNBits '%s': %zu scales, %lld expected", name, scales->data.size(), (long long)(N * groups));
+  if (zeros && (int64_t)zeros->data.size() != N * ceil_div(groups, 2)) OXB_DECLINE("MatMulNBits '%s': zero points must be packed, %lld bytes", name, (long long)(N * ceil_div(groups, 2)));
+  if (bias && (int64_t)bias->data.size() != N) OXB_DECLINE("MatMulNBits '%s': %zu bias lanes, %lld expected", name, bias->data.size(), (long long)N);
+  auto is_bytes = [](const HostTensor& t) {
+    for (float v : t.data)
+      if (!(v >= 0.f && v <= 255.f && v == std::floor(v))) return false;
+    return true;
+  };
+  if (!is_bytes(*codes) || (zeros && !is_bytes(*zeros))) OXB_DECLINE("MatMulNBits '%s': codes and zero points must be bytes", name);
+  int xi = typed_value_of(in_name(n, 0));
+  if (V(xi).shape.size() == 4 && V(xi).layout == Layout::NHWC && !order_free(V(xi))) xi = ensure_layout(n, xi, Layout::PLAIN);
+  const Value xv = V(xi);
+  if (xv.dt != DT::F32 && xv.dt != DT::F16 && xv.dt != DT::BF16) OXB_DECLINE("MatMulNBits '%s': x is %s", name, dt_name(xv.dt));
+  if (xv.shape.empty() || xv.shape.back() != K) OXB_DECLINE("MatMulNBits '%s': the last extent of x is not K", name);
+  std::vector<int64_t> os = xv.shape;
+  os.back() = N;
+
+  k::Linear4 a{};
+  a.rows = prod(xv.shape) / K;
+  a.k = (int)K, a.n = (int)N, a.group = (int)group, a.groups = (int)groups;
+  a.dt = xv.dt;
+  auto bytes_form = [&](const HostTensor* t, const std::string& of) {
+    return (uint8_t*)C.resident_form(of, "bytes", std::max<size_t>(t->data.size(), 16), [t](void* p) {
+      for (size_t i = 0; i < t->data.size(); ++i) ((uint8_t*)p)[i] = (uint8_t)t->data[i];
+    }, cacheable_const(of));
+  };
+  auto lanes_form = [&](const HostTensor* t, const std::string& of) {
+    return (const float*)C.resident_form(of, "raw_f32", std::max<size_t>(t->data.size() * 4, 4), [t](void* p) { std::memcpy(p, t->data.data(), t->data.size() * 4); },
+                                         cacheable_const(of));
+  };
+  a.codes = bytes_form(codes, in_name(n, 1));
+  a.scales = lanes_form(scales, in_name(n, 2));
+  if (zeros) a.zeros = bytes_form(zeros, in_name(n, 3));
+  if (bias) a.bias = lanes_form(bias, in_name(n, 5));
+
+  const int yi = add_typed(n.outputs[0], os, xv.dt);
+  V(yi).late_address = true;
+  Step& st = add_step(n, "linear4", 1, {xi}, {yi});
+  st.work = 2.0 * (double)a.rows * (double)K * (double)N;
+  st.work_is_bytes = false;
+  st.param_bytes = (double)codes->data.size() + 4.0 * (double)scales->data.size() + (zeros ? (double)zeros->data.size() : 0.0);
+  st.launch = [this, a, xi, yi](cudaStream_t s) {
+    k::Linear4 b = a;
+    b.x = V(xi).ptr;
+    b.y = V(yi).ptr;
+    k::linear4(b, s);
+    C.counters.simt_launches++;
+    C.counters.kernel_launches++;
+  };
+  widen(n, n.outputs[0]);
+}
+
+// What both operators over a paged cache share: inputs `first` .. `first` + 4 are key cache, value cache, cu_query,
+// kv_lengths, page_table.
+struct Planner::PagedInputs {
+  int kc, vc, cu, len, table;
+  int heads, kv_heads, size;
+  DT dt;
+  k::PagedTables t;
+  k::PagedTables bound(Planner& p) const {
+    k::PagedTables r = t;
+    r.cu_query = (const int*)p.V(cu).ptr;
+    r.kv_lengths = (const int*)p.V(len).ptr;
+    r.page_table = (const int*)p.V(table).ptr;
+    return r;
+  }
+};
+
+Planner::PagedInputs Planner::paged_inputs(const NodeDef& n, size_t first) {
+  const char *op = n.op.c_str(), *name = n.name.c_str();
+  for (size_t i = first; i < first + 5; ++i)
+    if (!has_in(n, i)) OXB_DECLINE("%s '%s': input %zu is missing", op, name, i);
+  PagedInputs r{};
+  r.kc = typed_value_of(in_name(n, first));
+  r.vc = typed_value_of(in_name(n, first + 1));
+  r.cu = typed_value_of(in_name(n, first + 2));
+  r.len = typed_value_of(in_name(n, first + 3));
+  r.table = typed_value_of(in_name(n, first + 4));
+  const Value &kv = V(r.kc), &vv = V(r.vc);
+  if ((kv.dt != DT::F16 && kv.dt != DT::BF16) || vv.dt != kv.dt) OXB_DECLINE("%s '%s': the caches must both be f16 or both bf16 (they are %s and %s)", op, name, dt_name(kv.dt), dt_name(vv.dt));
+  if (kv.shape.size() != 4 || kv.shape != vv.shape) OXB_DECLINE("%s '%s': the caches must both be [pages][page][kv_heads][size]", op, name);
+  r.heads = (int)n.attrs.i("num_heads", 0);
+  r.kv_heads = (int)n.attrs.i("kv_num_heads", 0);
+  r.dt = kv.dt;
+  if (r.kv_heads <= 0 || r.heads <= 0 || r.heads % r.kv_heads != 0 || kv.shape[2] != r.kv_heads || r.heads > 1024)
+    OXB_DECLINE("%s '%s': num_heads %d, kv_num_heads %d, caches of %lld heads", op, name, r.heads, r.kv_heads, (long long)kv.shape[2]);
+  if (kv.shape[3] <= 0 || kv.shape[3] % 8 != 0 || kv.shape[3] > 256) OXB_DECLINE("%s '%s': heads of %lld lanes (multiples of 8 up to 256)", op, name, (long long)kv.shape[3]);
+  r.size = (int)kv.shape[3];
+  if (kv.shape[1] <= 0 || kv.shape[1] % 16 != 0 || kv.shape[1] > 65536) OXB_DECLINE("%s '%s': pages of %lld tokens (multiples of 16)", op, name, (long long)kv.shape[1]);
+  if (kv.shape[0] <= 0 || kv.shape[0] > 0x7fffffff) OXB_DECLINE("%s '%s': a cache of %lld pages", op, name, (long long)kv.shape[0]);
+  for (int vi : {r.cu, r.len, r.table})
+    if (V(vi).dt != DT::I32) OXB_DECLINE("%s '%s': cu_query, kv_lengths and page_table must be declared i32 ('%s' is %s)", op, name, V(vi).name.c_str(), dt_name(V(vi).dt));
+  const int64_t sequences = V(r.len).numel();
+  if (sequences <= 0 || sequences > k::kMaxSequences || V(r.cu).numel() != sequences + 1) OXB_DECLINE("%s '%s': %lld lengths, %lld row bounds", op, name, (long long)sequences, (long long)V(r.cu).numel());
+  const std::vector<int64_t>& ts = V(r.table).shape;
+  if (ts.size() != 2 || ts[0] != sequences || ts[1] <= 0 || ts[1] * kv.shape[1] > 0x7fffffff) OXB_DECLINE("%s '%s': page_table must be [sequences][pages of a sequence]", op, name);
+  r.t.sequences = (int)sequences;
+  r.t.max_pages = (int)ts[1];
+  r.t.page = (int)kv.shape[1];
+  r.t.pages = kv.shape[0];
+  return r;
+}
+
+// OxiPagedCacheAppend: inputs query, key, value (the three or, with key and value omitted, one product [.., (heads + 2
+// kv_heads) * size]), key cache, value cache, cu_query, kv_lengths, page_table, optional cos and sin [positions][half].
+// Outputs: the rotated queries in the cache's type, and the caches, which are updated where they lie.
+void Planner::plan_paged_append(const NodeDef& n) {
+  check_attrs(n, {"num_heads", "kv_num_heads", "interleaved"});
+  const char* name = n.name.c_str();
+  PagedInputs p = paged_inputs(n, 3);
+  if (n.outputs.size() != 3 || n.outputs[0].empty() || n.outputs[1].empty() || n.outputs[2].empty()) OXB_DECLINE("OxiPagedCacheAppend '%s': three outputs", name);
+  if (p.kc == p.vc) OXB_DECLINE("OxiPagedCacheAppend '%s': one buffer for keys and values", name);
+  for (size_t i = 3; i < 5; ++i) {
+    auto it = consumers_.find(in_name(n, i));
+    int root = i == 3 ? p.kc : p.vc;
+    while (V(root).alias_of >= 0) root = V(root).alias_of;
+    if (!V(root).is_graph_input || V(root).host) OXB_DECLINE("OxiPagedCacheAppend '%s': a cache must be a graph input", name);
+    if (it->second.size() != 1 || graph_outputs_.count(in_name(n, i)))
+      OXB_DECLINE("OxiPagedCacheAppend '%s': '%s' is updated where it lies; what else reads it must read the output", name, in_name(n, i).c_str());
+  }
+  const bool packed = !has_in(n, 1) && !has_in(n, 2);
+  if (has_in(n, 1) != has_in(n, 2)) OXB_DECLINE("OxiPagedCacheAppend '%s': key without value", name);
+  int in[3] = {typed_value_of(in_name(n, 0)), -1, -1};
+  if (!packed)
+    for (int i = 1; i < 3; ++i) in[i] = typed_value_of(in_name(n, i));
+  const int64_t qw = (int64_t)p.heads * p.size, kw = (int64_t)p.kv_heads * p.size;
+  const Value qv = V(in[0]);
+  const int64_t tokens = qv.shape.empty() || qv.shape.back() == 0 ? 0 : qv.numel() / qv.shape.back();
+  for (int i = 0; i < (packed ? 1 : 3); ++i) {
+    if (V(in[i]).shape.size() == 4 && V(in[i]).layout == Layout::NHWC && !order_free(V(in[i]))) in[i] = ensure_layout(n, in[i], Layout::PLAIN);
+    const Value& v = V(in[i]);
+    const int64_t width = packed ? qw + 2 * kw : i == 0 ? qw : kw;
+    if (v.shape.size() < 2 || v.shape.back() != width || v.numel() != tokens * width) OXB_DECLINE("OxiPagedCacheAppend '%s': '%s' must be [tokens][%lld]", name, v.name.c_str(), (long long)width);
+    if (v.dt != qv.dt || (v.dt != DT::F32 && v.dt != p.dt)) OXB_DECLINE("OxiPagedCacheAppend '%s': '%s' is %s, the caches are %s (f32 or the caches' type, all alike)", name, v.name.c_str(), dt_name(v.dt), dt_name(p.dt));
+  }
+  if (tokens > 0x7fffffff / std::max(p.heads, 1)) OXB_DECLINE("OxiPagedCacheAppend '%s': %lld tokens", name, (long long)tokens);
+  if (has_in(n, 8) != has_in(n, 9)) OXB_DECLINE("OxiPagedCacheAppend '%s': cos without sin", name);
+  int cos = -1, sin = -1;
+  if (has_in(n, 8)) {
+    cos = value_of(in_name(n, 8)), sin = value_of(in_name(n, 9));
+    const Value &c = V(cos), &s = V(sin);
+    if (c.dt != DT::F32 || s.dt != DT::F32 || c.shape.size() != 2 || c.shape != s.shape || c.shape[1] < 1 || 2 * c.shape[1] > p.size)
+      OXB_DECLINE("OxiPagedCacheAppend '%s': cos and sin must be f32 [positions][half of the rotated lanes]", name);
+  }
+  k::PagedAppend a{};
+  a.t = p.t;
+  a.t.tokens = tokens;
+  a.q_stride = packed ? qw + 2 * kw : qw;
+  a.k_stride = a.v_stride = packed ? a.q_stride : kw;
+  if (cos >= 0) a.positions = V(cos).shape[0], a.half = (int)V(cos).shape[1];
+  a.heads = p.heads, a.kv_heads = p.kv_heads, a.size = p.size;
+  a.interleaved = n.attrs.i("interleaved", 0) != 0;
+  a.in_dt = qv.dt, a.cache_dt = p.dt;
+  a.err = S.err_flag_;
+  std::vector<int64_t> os = qv.shape;
+  os.back() = qw;
+  const int yi = add_typed(n.outputs[0], os, p.dt);
+  V(yi).late_address = true;
+  int outs[2];
+  for (int i = 0; i < 2; ++i) {
+    const int root = i == 0 ? p.kc : p.vc;
+    outs[i] = add_typed(n.outputs[1 + i], V(root).shape, p.dt);
+    V(outs[i]).alias_of = root;
+    V(outs[i]).ptr = V(root).ptr;
+  }
+  std::vector<int> reads = {in[0], p.kc, p.vc, p.cu, p.len, p.table};
+  for (int vi : {in[1], in[2], cos, sin})
+    if (vi >= 0) reads.push_back(vi);
+  const int lane = (int)dt_size(qv.dt);
+  const int qi = in[0], ki = in[1], vi = in[2];
+  Step& st = add_step(n, "paged_append", 2, reads, {yi, outs[0], outs[1]});
+  st.work = (double)tokens * (double)(qw + 2 * kw) * (double)(lane + 2);
+  st.launch = [this, a, p, qi, ki, vi, cos, sin, yi, qw, kw, lane](cudaStream_t s) {
+    k::PagedAppend b = a;
+    const PagedInputs& in = p;
+    const int64_t tokens = b.t.tokens;
+    b.t = in.bound(*this);
+    b.t.tokens = tokens;
+    b.q = V(qi).ptr;
+    b.k = ki >= 0 ? V(ki).ptr : (const uint8_t*)b.q + qw * lane;
+    b.v = vi >= 0 ? V(vi).ptr : (const uint8_t*)b.q + (qw + kw) * lane;
+    b.rotated = V(yi).ptr;
+    b.key_cache = V(in.kc).ptr;
+    b.value_cache = V(in.vc).ptr;
+    if (cos >= 0) b.cos = (const float*)V(cos).ptr, b.sin = (const float*)V(sin).ptr;
+    k::paged_append(b, s);
+    C.counters.glue_launches++;
+    C.counters.kernel_launches++;
+  };
+  for (const std::string& o : n.outputs) widen(n, o);
+}
+
+// OxiPagedAttention: inputs query [.., heads * size], key cache, value cache, cu_query, kv_lengths, page_table.  Row i of a
+// sequence's n new ones sees the tokens up to its own, kv_lengths - n + i.  The output has the caches' type; a query in f32
+// is rounded to it.
+void Planner::plan_paged_attention(const NodeDef& n) {
+  check_attrs(n, {"num_heads", "kv_num_heads", "scale", "max_query_length"});
+  const char* name = n.name.c_str();
+  const PagedInputs p = paged_inputs(n, 1);
+  if (n.outputs.size() != 1) OXB_DECLINE("OxiPagedAttention '%s': one output", name);
+  int qi = typed_value_of(in_name(n, 0));
+  if (V(qi).shape.size() == 4 && V(qi).layout == Layout::NHWC && !order_free(V(qi))) qi = ensure_layout(n, qi, Layout::PLAIN);
+  const int64_t qw = (int64_t)p.heads * p.size;
+  if (V(qi).shape.size() < 2 || V(qi).shape.back() != qw) OXB_DECLINE("OxiPagedAttention '%s': query must be [tokens][%lld]", name, (long long)qw);
+  if (V(qi).dt != DT::F32 && V(qi).dt != p.dt) OXB_DECLINE("OxiPagedAttention '%s': the query is %s, the caches are %s", name, dt_name(V(qi).dt), dt_name(p.dt));
+  const std::vector<int64_t> os = V(qi).shape;
+  if (V(qi).dt == DT::F32) qi = half_copy(n, qi, p.dt);
+  k::PagedAttention a{};
+  a.t = p.t;
+  a.t.tokens = prod(os) / qw;
+  if (a.t.tokens > 0x7fffffff / p.heads) OXB_DECLINE("OxiPagedAttention '%s': %lld tokens", name, (long long)a.t.tokens);
+  a.heads = p.heads, a.kv_heads = p.kv_heads, a.size = p.size;
+  a.scale = n.attrs.f("scale", 1.0f / std::sqrt((float)p.size));
+  const int64_t most = n.attrs.i("max_query_length", 0);
+  if (!std::isfinite(a.scale) || most < 0) OXB_DECLINE("OxiPagedAttention '%s': scale %g, max_query_length %lld", name, (double)a.scale, (long long)most);
+  a.max_query = (int)std::min<int64_t>(most, a.t.tokens);
+  a.dt = p.dt;
+  a.err = S.err_flag_;
+  if (const size_t bytes = k::paged_attention_workspace(a)) {
+    a.workspace = owned_buffer(bytes);
+    OXB_CUDA(cudaMemsetAsync(a.workspace, 0, bytes, C.stream()));
+    OXB_CUDA(cudaStreamSynchronize(C.stream()));
+  }
+  const int yi = add_typed(n.outputs[0], os, p.dt);
+  V(yi).late_address = true;
+  Step& st = add_step(n, "paged_attention", 0, {qi, p.kc, p.vc, p.cu, p.len, p.table}, {yi});
+  st.late_address = true;
+  st.work = 2.0 * (double)V(yi).bytes;
+  st.launch = [this, a, p, qi, yi](cudaStream_t s) {
+    k::PagedAttention b = a;
+    b.t = p.bound(*this);
+    b.t.tokens = a.t.tokens;
+    b.q = V(qi).ptr;
+    b.key_cache = V(p.kc).ptr;
+    b.value_cache = V(p.vc).ptr;
+    b.out = V(yi).ptr;
+    k::paged_attention(b, s);
+    C.counters.umma_launches++;
+    C.counters.kernel_launches++;
+  };
+  widen(n, n.outputs[0]);
+}
+
 // Transpose (shape/basic.rs:146): any permutation of up to four logical axes of a 32-bit tensor.
 void Planner::plan_transpose(const NodeDef& n) {
   check_attrs(n, {"perm"});
@@ -3460,7 +3796,8 @@ void Planner::plan_layer_norm(const NodeDef& n) {
 // shares the input's storage.  A channels-last activation whose order matters is first brought
 // back to the logical order; int32 lanes cast to float become f32 lanes (round to nearest even).
 void Planner::plan_alias(const NodeDef& n) {
-  int xi = value_of(in_name(n, 0));
+  const bool keeps_type = n.op != "Cast" && typed_index_.count(in_name(n, 0));
+  int xi = keeps_type ? typed_value_of(in_name(n, 0)) : value_of(in_name(n, 0));
   std::vector<int64_t> os;
   const Value xv0 = V(xi);
   if (n.op == "Flatten") {
@@ -3527,10 +3864,11 @@ void Planner::plan_alias(const NodeDef& n) {
   const Value xv = V(xi);
   Layout ol = Layout::PLAIN;
   if (os.size() == 4) ol = shape_changes ? Layout::PLAIN : xv.layout;
-  int yi = add_value(n.outputs[0], os, xv.dt, ol);
+  int yi = keeps_type ? add_typed(n.outputs[0], os, xv.dt) : add_value(n.outputs[0], os, xv.dt, ol);
   V(yi).alias_of = xi;
   V(yi).host = xv.host;
   if (xv.external && xv.ptr) V(yi).ptr = xv.ptr;
+  if (keeps_type) widen(n, n.outputs[0]);
 }
 
 // DequantizeLinear(a) , DequantizeLinear(b) -> Add -> Relu -> QuantizeLinear with per-tensor

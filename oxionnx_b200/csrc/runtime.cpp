@@ -402,6 +402,8 @@ void Context::device_to_host(void* dst, const void* src, size_t bytes, cudaStrea
 Session::~Session() {
   cudaSetDevice(ctx_->device());
   cudaStreamSynchronize(ctx_->stream());
+  if (enqueued_) cudaEventSynchronize(enqueued_ev_);
+  if (enqueued_ev_) cudaEventDestroy(enqueued_ev_);
   for (auto* p : umma_plans_) k::umma_plan_destroy(p);
   for (auto* g : umma_groups_) k::umma_group_destroy(g);
   for (auto* c : umma_chains_) k::umma_chain_destroy(c);
@@ -478,6 +480,7 @@ static const void* feed_lanes(const oxb200_operand& f, const Value& v, const cha
 
 // A run that failed half way leaves copies in the staging memory that nobody will collect.
 void Session::begin_copies() {
+  follow_enqueued(ctx_->stream());
   if (small_stage_used_ == 0 && pending_out_.empty()) return;
   pending_out_.clear();
   OXB_CUDA(cudaStreamSynchronize(ctx_->stream()));
@@ -559,7 +562,18 @@ void Session::stage_out(void* dst, const void* src, size_t bytes) {
   OXB_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToHost, ctx_->stream()));
 }
 
-bool Session::capture_graph(GraphSlot& g) {
+// Orders stream `s` behind the last run that was enqueued on a caller's stream.
+void Session::follow_enqueued(cudaStream_t s) {
+  if (!enqueued_ || enqueued_on_ == s) return;
+  OXB_CUDA(cudaStreamWaitEvent(s, enqueued_ev_, 0));
+  if (s == ctx_->stream()) enqueued_ = false;
+}
+
+static bool skipped(const Step& st, bool lanes_wanted, const std::vector<char>& typed) {
+  return !lanes_wanted && st.host_copy_of >= 0 && typed[st.host_copy_of];
+}
+
+bool Session::capture_graph(GraphSlot& g, bool lanes_wanted) {
   cudaStream_t s = ctx_->stream();
   const oxb200_counters before = ctx_->counters;
   if (cudaStreamBeginCapture(s, cudaStreamCaptureModeThreadLocal) != cudaSuccess) {
@@ -568,7 +582,10 @@ bool Session::capture_graph(GraphSlot& g) {
   }
   bool ok = true;
   try {
-    for (auto& st : steps_) st.launch(s);
+    std::vector<char> typed(outputs_.size(), 0);
+    for (const auto& kv : bound_out_) typed[kv.first] = kv.second.typed;
+    for (auto& st : steps_)
+      if (!skipped(st, lanes_wanted, typed)) st.launch(s);
   } catch (...) {
     ok = false;
   }
@@ -590,9 +607,15 @@ bool Session::capture_graph(GraphSlot& g) {
   return ok;
 }
 
-bool Session::replay_graph() {
+bool Session::replay_graph(bool lanes_wanted, cudaStream_t stream) {
   std::vector<void*> key;
   for (auto& in : input_staging_) key.push_back(values_[in.second].ptr);
+  for (size_t i = 0; i < output_raw_.size(); ++i) {  // outputs that are written to a caller's buffer, and whose f32 lanes are left out
+    auto b = bound_out_.find((int)i);
+    if (b == bound_out_.end() || !b->second.typed) continue;
+    key.push_back((void*)(uintptr_t)(i * 2 + (lanes_wanted ? 1 : 0)));
+    key.push_back(values_[output_value((int)i, true)].ptr);
+  }
   GraphSlot* g = nullptr;
   for (auto& c : graphs_)
     if (c.key == key) g = &c;
@@ -609,14 +632,14 @@ bool Session::replay_graph() {
       g->warmed = true;
       return false;
     }
-    if (!capture_graph(*g)) {
+    if (!capture_graph(*g, lanes_wanted)) {
       g->poisoned = true;
       ctx_->counters.graph_poisoned += 1;
       return false;
     }
     ctx_->counters.graph_captures += 1;
   }
-  OXB_CUDA(cudaGraphLaunch(g->exec, ctx_->stream()));
+  OXB_CUDA(cudaGraphLaunch(g->exec, stream));
   ctx_->counters.graph_replays += 1;
   ctx_->counters.kernel_launches += g->d_kernel;
   ctx_->counters.umma_launches += g->d_umma;
@@ -626,10 +649,18 @@ bool Session::replay_graph() {
   return true;
 }
 
-void Session::run_steps(bool profile) {
-  cudaStream_t s = ctx_->stream();
-  if (graph_allowed_ && !profile && ctx_->cfg().cuda_graph && !ctx_->cfg().verify && replay_graph()) return;
+void Session::run_steps(bool profile, bool lanes_wanted, cudaStream_t s) {
+  const bool on_own_stream = s == nullptr;
+  if (on_own_stream) {
+    s = ctx_->stream();
+    follow_enqueued(s);
+  }
+  // recordings are made and replayed on the context's stream; a caller that wants one of its own stream captures it itself
+  if (graph_allowed_ && !profile && ctx_->cfg().cuda_graph && !ctx_->cfg().verify && on_own_stream && replay_graph(lanes_wanted, s)) return;
+  std::vector<char> typed(outputs_.size(), 0);
+  for (const auto& kv : bound_out_) typed[kv.first] = kv.second.typed;
   for (auto& st : steps_) {
+    if (skipped(st, lanes_wanted, typed)) continue;
     if (profile) {
       if (!st.ev0) {
         OXB_CUDA(cudaEventCreate(&st.ev0));
@@ -656,11 +687,22 @@ void Session::download(oxb200_result* fetches, uint32_t n) {
   finish_download();
 }
 
+// What the kernels' error word says; every text takes the code.
+static const char* error_text(int flag) {
+  switch (flag) {
+    case 20: return "Gather: an index is out of range (device code %d); results are not valid";
+    case 21: return "paged cache: an entry of the page table that a sequence needs is no page of the cache (device code %d); what needed it was skipped";
+    case 22: return "paged cache: a token's position has no row in cos / sin (device code %d); the token was skipped";
+    case 23: return "paged cache: cu_query does not rise from 0 to the number of query rows, or a length exceeds the page table (device code %d); results are not valid";
+    case 24: return "OxiPagedAttention: a sequence has more query rows than max_query_length (device code %d); results are not valid";
+    default: return "a tensor-core kernel gave up on a bounded wait (code %d); results are not valid";
+  }
+}
+
 void Session::finish_download() {
   sync();
   int flag = check_error_flag();
-  if (flag)
-    raise(OXB200_FAILED, flag == 20 ? "Gather: an index is out of range (device code %d); results are not valid" : "a tensor-core kernel gave up on a bounded wait (code %d); results are not valid", flag);
+  if (flag) raise(OXB200_FAILED, error_text(flag), flag);
 }
 
 void Session::download_async(oxb200_result* fetches, uint32_t n) {
@@ -689,6 +731,8 @@ void Session::fetch_value(const std::string& name, oxb200_result* out) {
   if (!v->ptr) raise(OXB200_FAILED, "fetch_value: '%s' has no device storage (fused away)", name.c_str());
   write_result_shape(*v, out);
   if (!out->lanes) return;
+  require_not_typed(name);
+  follow_enqueued(ctx_->stream());
   if (out->cap < (uint64_t)v->numel()) raise(OXB200_FAILED, "fetch_value: buffer too small for '%s'", name.c_str());
   int64_t n = v->numel();
   if (n == 0) return;
@@ -735,7 +779,7 @@ void Session::prepare_pipeline() {
   // the tensor-core steps are the ones that do, so none of them may read an input (or an alias of one).
   pipe_double_ = external_bind_.empty();
   for (const Step& st : steps_) {
-    if (st.family != 0) continue;
+    if (st.family != 0 || st.late_address) continue;
     for (int r : st.reads) {
       int root = r;
       while (values_[root].alias_of >= 0) root = values_[root].alias_of;
@@ -880,7 +924,7 @@ size_t Session::device_bytes() const {
 bool Session::input_in_tensor_map(int value_index) const {
   // the tensor-core steps build their operands' addresses into tensor maps at plan time
   for (const Step& st : steps_) {
-    if (st.family != 0) continue;
+    if (st.family != 0 || st.late_address) continue;
     for (int r : st.reads) {
       int root = r;
       while (values_[root].alias_of >= 0) root = values_[root].alias_of;
@@ -907,21 +951,74 @@ void Session::bind_input_device(const std::string& name, const void* ptr, DT dt,
   raise(OXB200_FAILED, "bind_input_device: '%s' is not an input of the planned graph", name.c_str());
 }
 
-void Session::bind_output_device(const std::string& name, void* ptr, uint64_t cap) {
+void Session::bind_output_device(const std::string& name, void* ptr, uint64_t cap, bool typed, DT dt) {
   for (size_t i = 0; i < output_staging_.size(); ++i) {
     if (output_staging_[i].first != name) continue;
-    const Value& v = values_[output_staging_[i].second];
+    const Value& v = values_[output_value((int)i, typed)];
+    if (dt != v.dt) raise(OXB200_FAILED, "bind_output_device: '%s' was planned as %s, the buffer is %s", name.c_str(), dt_name(v.dt), dt_name(dt));
     if (cap < (uint64_t)v.numel()) raise(OXB200_FAILED, "bind_output_device: '%s' has %lld lanes, the buffer holds %llu", name.c_str(), (long long)v.numel(), (unsigned long long)cap);
-    if (!ptr || ((uintptr_t)ptr & 3) != 0) raise(OXB200_FAILED, "bind_output_device: the buffer of '%s' must be a 4-byte aligned device address", name.c_str());
-    bound_out_[(int)i] = {ptr, cap};
+    const size_t lane = dt_size(dt);
+    if (!ptr || ((uintptr_t)ptr & (lane - 1)) != 0) raise(OXB200_FAILED, "bind_output_device: the buffer of '%s' must be a %zu-byte aligned device address", name.c_str(), lane);
+    bound_out_[(int)i] = BoundOutput{ptr, typed};
     return;
   }
   raise(OXB200_FAILED, "bind_output_device: '%s' is not an output of the planned graph", name.c_str());
 }
 
+bool Session::overlaps_own_memory(const void* p, size_t bytes) const {
+  auto meets = [&](const void* q, size_t n) { return q && (const uint8_t*)p < (const uint8_t*)q + n && (const uint8_t*)q < (const uint8_t*)p + bytes; };
+  if (meets(arena_.ptr, arena_.bytes)) return true;
+  for (const DeviceBuffer& b : owned_)
+    if (meets(b.ptr, b.bytes)) return true;
+  for (const auto& in : input_staging_)
+    if (meets(values_[in.second].ptr, values_[in.second].bytes)) return true;
+  return false;
+}
+
+// A typed output is written where it was bound when its step takes the address at each launch, nothing else of the run
+// lies there, and the address suits 16-byte stores; otherwise it is copied there behind the steps.
+void Session::point_outputs() {
+  for (auto& kv : bound_out_) {
+    if (!kv.second.typed) continue;
+    Value& v = values_[output_value(kv.first, true)];
+    if (!v.late_address || v.numel() == 0 || ((uintptr_t)kv.second.ptr & 15) != 0 || kv.second.ptr == v.ptr || overlaps_own_memory(kv.second.ptr, v.bytes)) continue;
+    bool alone = true;
+    for (const Value& view : values_) {  // views of it hold its address
+      const Value* root = &view;
+      while (root->alias_of >= 0) root = &values_[root->alias_of];
+      alone = alone && (root != &v || &view == &v);
+    }
+    for (const auto& other : bound_out_) {
+      if (other.first == kv.first) continue;
+      const Value& w = values_[output_value(other.first, other.second.typed)];
+      const uint8_t *p = (const uint8_t*)kv.second.ptr, *q = (const uint8_t*)other.second.ptr;
+      alone = alone && &w != &v && !(p < q + w.bytes && q < p + v.bytes);
+    }
+    if (!alone) continue;
+    kv.second.own = v.ptr;
+    v.ptr = kv.second.ptr;
+  }
+}
+
+void Session::restore_outputs() {
+  for (auto& kv : bound_out_)
+    if (kv.second.own) {
+      values_[output_value(kv.first, true)].ptr = kv.second.own;
+      kv.second.own = nullptr;
+    }
+}
+
+// The f32 lanes of an output that the last runs wrote to a caller's buffer are not here.
+void Session::require_not_typed(const std::string& name) const {
+  for (const auto& kv : bound_out_)
+    if (kv.second.typed && output_staging_[kv.first].first == name)
+      raise(OXB200_FAILED, "'%s' is bound to a device buffer in its own type; read it there", name.c_str());
+}
+
 void Session::output_device_ptr(const std::string& name, void** ptr, uint64_t* len) {
   for (size_t i = 0; i < output_staging_.size(); ++i) {
     if (output_staging_[i].first != name) continue;
+    require_not_typed(name);
     const Value& v = values_[output_staging_[i].second];
     if (ptr) *ptr = v.ptr;
     if (len) *len = (uint64_t)v.numel();
@@ -949,7 +1046,7 @@ static void copy_on_device(void* dst, const void* src, size_t bytes, cudaStream_
 
 // A bound input is read in place when no tensor map holds its buffer's address; otherwise its lanes are copied
 // device-to-device into the buffer the maps were built for (no host traffic either way).
-void Session::apply_input_bindings() {
+void Session::apply_input_bindings(cudaStream_t s) {
   if (in_tensor_map_.empty())
     for (auto& in : input_staging_) in_tensor_map_.push_back(input_in_tensor_map(in.second) ? 1 : 0);
   for (auto& kv : bound_in_) {
@@ -957,11 +1054,52 @@ void Session::apply_input_bindings() {
     Value& v = values_[vi];
     if (in_tensor_map_[kv.first]) {
       if (v.ptr != own_in_ptr_[kv.first]) rebind_input(vi, own_in_ptr_[kv.first]);
-      copy_on_device(v.ptr, kv.second, (size_t)v.numel() * dt_size(v.dt), ctx_->stream());
+      copy_on_device(v.ptr, kv.second, (size_t)v.numel() * dt_size(v.dt), s);
     } else {
       rebind_input(vi, const_cast<void*>(kv.second));
     }
   }
+}
+
+void Session::copy_outputs(cudaStream_t s) {
+  for (auto& kv : bound_out_) {
+    const Value& v = values_[output_value(kv.first, kv.second.typed)];
+    if (v.numel() > 0 && kv.second.ptr != v.ptr) copy_on_device(kv.second.ptr, v.ptr, (size_t)v.numel() * dt_size(v.dt), s);
+  }
+}
+
+void Session::enqueue(cudaStream_t stream) {
+  if (in_flight() > 0) raise(OXB200_FAILED, "run_enqueue: pipelined runs are in flight; collect them first");
+  if (!stream) stream = cudaStreamLegacy;  // the default stream by its own handle: null means the context's stream below
+  for (size_t i = 0; i < input_staging_.size(); ++i)
+    if (!bound_in_.count((int)i)) raise(OXB200_FAILED, "run_enqueue: graph input '%s' is not bound to a device buffer", input_staging_[i].first.c_str());
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  OXB_CUDA(cudaStreamIsCapturing(stream, &capturing));
+  const bool recorded = capturing != cudaStreamCaptureStatusNone;
+  if (!enqueued_ev_ && !recorded) OXB_CUDA(cudaEventCreateWithFlags(&enqueued_ev_, cudaEventDisableTiming));
+  if (!recorded) follow_enqueued(stream);
+  apply_input_bindings(stream);
+  point_outputs();
+  try {
+    run_steps(false, false, stream);
+    copy_outputs(stream);
+  } catch (...) {
+    restore_outputs();
+    throw;
+  }
+  restore_outputs();
+  if (recorded) return;
+  OXB_CUDA(cudaEventRecord(enqueued_ev_, stream));
+  enqueued_on_ = stream;
+  enqueued_ = true;
+}
+
+void Session::run_wait() {
+  if (enqueued_) {
+    OXB_CUDA(cudaEventSynchronize(enqueued_ev_));
+    enqueued_ = false;
+  }
+  finish_download();
 }
 
 void Session::run_bound(const oxb200_operand* feeds, uint32_t n, oxb200_result* fetches, uint32_t nf, bool profile) {
@@ -983,13 +1121,18 @@ void Session::run_bound(const oxb200_operand* feeds, uint32_t n, oxb200_result* 
     ctx_->counters.uploads += 1;
     ctx_->counters.upload_bytes += (uint64_t)v.numel() * dt_size(v.dt);
   }
-  apply_input_bindings();
-  run_steps(profile);
-  for (auto& kv : bound_out_) {
-    const Value& v = values_[output_staging_[kv.first].second];
-    if (v.numel() > 0 && kv.second.first != v.ptr)
-      copy_on_device(kv.second.first, v.ptr, (size_t)v.numel() * 4, ctx_->stream());
+  bool lanes_wanted = false;  // somebody reads f32 lanes: nothing is written to a buffer in place of the session's own
+  for (uint32_t i = 0; fetches && i < nf; ++i) lanes_wanted = lanes_wanted || fetches[i].lanes;
+  apply_input_bindings(ctx_->stream());
+  if (!lanes_wanted) point_outputs();
+  try {
+    run_steps(profile, lanes_wanted);
+    copy_outputs(ctx_->stream());
+  } catch (...) {
+    restore_outputs();
+    throw;
   }
+  restore_outputs();
   if (fetches) {
     for (uint32_t i = 0; i < nf; ++i) {
       const Value& v = values_[output_staging_[i].second];

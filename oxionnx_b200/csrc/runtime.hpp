@@ -89,12 +89,15 @@ struct Value {
   int dq_src = -1, dq_step = -1;
   int out_seq = 0;  // > 0: the contraction that produces it writes its rows transposed within sequences of this many
   float dq_scale = 1.f, dq_zp = 0.f;
+  bool late_address = false;  // the step that writes it takes its address at each launch, so a run may point it at a caller's buffer
   int64_t numel() const { return prod(shape); }
 };
 
 struct Step {
   std::string node_name, op_type, kernel;
   int family = 2;  // 0 tcgen05, 1 direct CUDA-core, 2 glue
+  bool late_address = false;  // a tcgen05 step that builds its tensor maps at each launch: its inputs may move between runs
+  int host_copy_of = -1;      // >= 0: makes the f32 lanes of that graph output, which nobody reads while it is bound in its own type
   double work = 0;
   bool work_is_bytes = true;
   // algorithmic bytes of one launch: every value the step reads and writes once, plus `param_bytes` (a
@@ -124,7 +127,11 @@ class Session {
   void plan(const std::vector<NodeDef>& nodes, const std::vector<std::pair<std::string, std::vector<int64_t>>>& inputs,
             const std::map<std::string, const HostTensor*>& volatile_consts, const std::vector<std::string>& outputs);
   void upload(const oxb200_operand* feeds, uint32_t n);
-  void run_steps(bool profile);
+  // `lanes_wanted` false: outputs bound in their own type need no f32 lanes.
+  void run_steps(bool profile, bool lanes_wanted = true) { run_steps(profile, lanes_wanted, nullptr); }
+  // One run of a session whose inputs are all bound, on the caller's stream and without a fence; run_wait() is the fence.
+  void enqueue(cudaStream_t stream);
+  void run_wait();
   void download(oxb200_result* fetches, uint32_t n);
   void download_async(oxb200_result* fetches, uint32_t n);  // enqueue the copies
   void finish_download();                                    // one fence + the kernels' error word
@@ -141,7 +148,8 @@ class Session {
   void declare_input_type(const std::string& name, DT dt) { input_types_[name] = dt; }
   // Device I/O binding (after plan()): inputs read from, outputs also written to, caller-owned device buffers.
   void bind_input_device(const std::string& name, const void* ptr, DT dt, uint64_t len);
-  void bind_output_device(const std::string& name, void* ptr, uint64_t cap);
+  // `typed`: the lanes go to the buffer alone, in `dt`, the type that the graph gives the output.
+  void bind_output_device(const std::string& name, void* ptr, uint64_t cap, bool typed = false, DT dt = DT::F32);
   void output_device_ptr(const std::string& name, void** ptr, uint64_t* len);
   void clear_bindings();
   // run_with_binding: uploads the unbound inputs, runs, copies bound outputs device-to-device, downloads the
@@ -151,7 +159,7 @@ class Session {
   void use_resident(const std::string& name, const void* ptr);  // read in place, or copied when a tensor map holds the input's address
   void use_host(const std::string& name, const void* lanes);
   size_t device_bytes() const;
-  void begin_copies();
+  void begin_copies();  // before the context's stream touches the session's memory
   // After a run, detach the storage of an output so it can outlive the session.
   Value* find_value(const std::string& name);
   int check_error_flag();
@@ -185,10 +193,28 @@ class Session {
   // that buffer's address, read in place otherwise); output index -> caller's buffer and capacity
   std::map<int, const void*> bound_in_;
   std::vector<char> in_tensor_map_;  // per graph input: does a tensor map hold its buffer's address (filled at the first binding)
-  std::map<int, std::pair<void*, uint64_t>> bound_out_;
+  struct BoundOutput {
+    void* ptr;
+    bool typed;
+    void* own = nullptr;  // while a run writes the caller's buffer directly: the session's address of the value
+  };
+  std::map<int, BoundOutput> bound_out_;
+  std::vector<int> output_raw_;  // per graph output: its value in the graph's own 16-bit type, or -1
+  int output_value(int output, bool typed) const { return typed && output_raw_[output] >= 0 ? output_raw_[output] : output_staging_[output].second; }
+  void point_outputs();    // typed outputs that may be written in place of the session's own storage
+  void restore_outputs();
+  void copy_outputs(cudaStream_t s);
+  bool overlaps_own_memory(const void* p, size_t bytes) const;
+  void require_not_typed(const std::string& name) const;
+  void run_steps(bool profile, bool lanes_wanted, cudaStream_t stream);
+  // Runs on callers' streams: the last one's end, which any other stream waits for before it touches the session's memory.
+  cudaEvent_t enqueued_ev_ = nullptr;
+  cudaStream_t enqueued_on_ = nullptr;
+  bool enqueued_ = false;
+  void follow_enqueued(cudaStream_t s);
   std::vector<void*> own_in_ptr_;  // the session's own buffer of each graph input (what an unbound input reads)
   bool input_in_tensor_map(int value_index) const;
-  void apply_input_bindings();
+  void apply_input_bindings(cudaStream_t s);
   // Host lanes <-> device through page-locked staging (see stage_in / stage_out in runtime.cpp).
   uint8_t* small_stage_ = nullptr;  // small feeds, then small fetches, of the one synchronous run
   size_t small_stage_bytes_ = 0, small_stage_used_ = 0;
@@ -229,8 +255,8 @@ class Session {
   };
   std::vector<GraphSlot> graphs_;
   bool graph_allowed_ = false;
-  bool replay_graph();
-  bool capture_graph(GraphSlot& g);
+  bool replay_graph(bool lanes_wanted, cudaStream_t stream);
+  bool capture_graph(GraphSlot& g, bool lanes_wanted);
 
  public:
   void allow_graph(bool on) { graph_allowed_ = on; }

@@ -349,7 +349,8 @@ class SessionBuilder:
 
     def with_input_types(self, types: Dict[str, object]):
         """Declared element types of graph inputs (TensorInfo.dtype): np.uint8 / np.int8 inputs are stored, fed and
-        bound as 8-bit lanes instead of f32 lanes."""
+        bound as 8-bit lanes instead of f32 lanes, and inputs declared "float16", "bfloat16" or "int32" (by name; other
+        numpy types leave an input f32 lanes) in that type, for the decoder operators that read them."""
         self._input_types = dict(types)
         return self
 
@@ -379,16 +380,10 @@ class SessionBuilder:
         return Session.from_model(Model.from_file(path), self._device, 1 if level is None else level, self._input_shapes, **self._ctx_kw)
 
 
-def _lanes(feeds, names):
-    """The feeds of `names` as arrays the library reads in place: contiguous, 8-bit lanes as they are, anything else as
-    f32."""
-    lanes = {}
-    for name in names:
-        if name in feeds:
-            a = feeds[name]
-            typed = isinstance(a, np.ndarray) and a.dtype in _ffi.TYPED
-            lanes[name] = np.ascontiguousarray(a if typed else np.asarray(a, dtype=np.float32))
-    return lanes
+def _lanes(feeds, names, types):
+    """The feeds of `names` as arrays the library reads in place: contiguous, 8-bit lanes as they are, in the declared type
+    where an input was declared f16, bf16 or i32, anything else as f32."""
+    return {name: _ffi.lanes_of(feeds[name], _ffi.dtype_code(types[name]) if name in types else _ffi.DT_F32) for name in names if name in feeds}
 
 
 class _CallIo:
@@ -404,6 +399,7 @@ class _CallIo:
         self.feeds = (_ffi.RawOperand * max(self.n_in, 1))()
         self.feeds_ptr = ctypes.cast(self.feeds, ctypes.POINTER(_ffi.Operand))
         self.inputs = []
+        self.codes = {name: _ffi.dtype_code(t) for name, t in session._input_types.items()}
         for op, name in zip(self.feeds, graph.input_names):
             shape = planned[name]
             op.name = name.encode()
@@ -428,7 +424,8 @@ class _CallIo:
             a = lanes[name]
             if a.shape != shape and not (shape == () and a.size == 1):
                 raise OnnxError(f"run: feed '{name}' has shape {a.shape}, the plan expects {shape}")
-            typed = _ffi.TYPED.get(a.dtype)
+            typed = self.codes.get(name, _ffi.DT_F32)
+            typed = typed if typed in (_ffi.DT_F16, _ffi.DT_BF16, _ffi.DT_I32) else _ffi.TYPED.get(a.dtype)
             if typed is None:
                 op.lanes, op.typed = a.ctypes.data, None
             else:
@@ -485,7 +482,8 @@ class Session:
         for name, shape, _ in model.inputs():
             if name not in self._input_shapes and all(d is not None for d in shape):
                 self._input_shapes[name] = tuple(shape)
-        self._input_types = {name: (np.uint8 if code == _ffi.DT_U8 else np.int8) for name, _, code in model.inputs() if code in (_ffi.DT_U8, _ffi.DT_I8)}
+        by_code = {code: t for t, code in _ffi.NAMED.items() if code != _ffi.DT_F32}
+        self._input_types = {name: by_code[code] for name, _, code in model.inputs() if code in by_code}
         self._planned_for = None
         self._io = None
         self._in_flight = []
@@ -511,7 +509,7 @@ class Session:
             sh = shapes[name]
             ins[i].shape = keep.add((ctypes.c_uint64 * max(len(sh), 1))(*sh))
             ins[i].rank = len(sh)
-            ins[i].dtype = _ffi.TYPED.get(np.dtype(self._input_types[name]), _ffi.DT_F32) if name in self._input_types else _ffi.DT_F32
+            ins[i].dtype = _ffi.dtype_code(self._input_types[name]) if name in self._input_types else _ffi.DT_F32
         outs = keep.add((ctypes.c_char_p * max(len(self.graph.output_names), 1))(*[s.encode() for s in self.graph.output_names]))
         st = lib.oxb200_session_plan(self.ctx.handle, nodes, len(self.graph.nodes), ins, len(self.graph.input_names), outs,
                                      len(self.graph.output_names))
@@ -548,7 +546,7 @@ class Session:
         return self._io
 
     def run(self, feeds: Dict[str, np.ndarray]) -> Dict[str, np.ndarray]:
-        lanes = _lanes(feeds, self.graph.input_names)
+        lanes = _lanes(feeds, self.graph.input_names, self._input_types)
         with self._lock:
             self.ensure_planned(feeds)
             io = self._call_io()
@@ -563,7 +561,7 @@ class Session:
     def submit(self, feeds: Dict[str, np.ndarray]):
         """Enqueues one run (upload, steps, download) and returns at once; at most two may be in flight.
         The feed arrays must stay unchanged until the matching collect()."""
-        lanes = _lanes(feeds, self.graph.input_names)
+        lanes = _lanes(feeds, self.graph.input_names, self._input_types)
         with self._lock:
             self.ensure_planned(feeds)
             io = self._call_io()
@@ -602,14 +600,18 @@ class Session:
     # ---- device I/O binding (IoBinding / run_with_binding, extended to device memory) ----
     def bind_input_device(self, name: str, device_ptr: int, dtype, count: int):
         """Graph input `name` is read from the caller's device buffer by the following runs."""
-        code = _ffi.TYPED.get(np.dtype(dtype), _ffi.DT_F32)
+        code = _ffi.dtype_code(dtype)
         st = _ffi.lib().oxb200_bind_input_device(self.ctx.handle, name.encode(), device_ptr, code, count)
         if st:
             _raise_for(st, self.ctx.last_error())
 
-    def bind_output_device(self, name: str, device_ptr: int, capacity: int):
-        """Graph output `name` (f32 lanes, logical order) is also written to the caller's device buffer."""
-        st = _ffi.lib().oxb200_bind_output_device(self.ctx.handle, name.encode(), device_ptr, capacity)
+    def bind_output_device(self, name: str, device_ptr: int, capacity: int, dtype: Optional[str] = None):
+        """Graph output `name` (f32 lanes, logical order) is also written to the caller's device buffer; with `dtype`
+        ("float32", "float16", "bfloat16": the type the graph gives the output) it is written there alone, in that type."""
+        if dtype is None:
+            st = _ffi.lib().oxb200_bind_output_device(self.ctx.handle, name.encode(), device_ptr, capacity)
+        else:
+            st = _ffi.lib().oxb200_bind_output_device_typed(self.ctx.handle, name.encode(), device_ptr, _ffi.dtype_code(dtype), capacity)
         if st:
             _raise_for(st, self.ctx.last_error())
 
@@ -633,7 +635,9 @@ class Session:
         names = [n for n in self.graph.input_names if n in feeds]
         ops = keep.add((_ffi.Operand * max(len(names), 1))())
         for i, name in enumerate(names):
-            _ffi.pack_operand(ops[i], name, feeds[name], keep)
+            code = _ffi.dtype_code(self._input_types[name]) if name in self._input_types else _ffi.DT_F32
+            typed = code if code in (_ffi.DT_F16, _ffi.DT_BF16, _ffi.DT_I32) else _ffi.DT_F32
+            _ffi.pack_operand(ops[i], name, _ffi.lanes_of(feeds[name], code), keep, dtype=typed)
         if not fetch:
             _raise_for(lib.oxb200_run_bound(self.ctx.handle, ops, len(names), None, 0), self.ctx.last_error())
             return None
@@ -643,12 +647,28 @@ class Session:
             _raise_for(lib.oxb200_run_bound(self.ctx.handle, ops, len(names), io.fetches_ptr, io.n_out), self.ctx.last_error())
         return outs
 
+    def enqueue(self, stream: int = 0):
+        """One run with every input bound, put into a CUDA stream (its handle, 0: the default stream) without waiting for
+        it: outputs are in their bound buffers when the stream gets there.  Runs of one session follow one another.  What
+        the kernels found wrong is reported by wait() or the next call that waits."""
+        st = self._enqueue(self.ctx.handle, stream)
+        if st > _ffi.OK_DEVICE:
+            _raise_for(st, self.ctx.last_error())
+
+    @property
+    def _enqueue(self):
+        return _ffi.lib().oxb200_run_enqueue
+
+    def wait(self):
+        """Waits for the enqueued runs and raises what their kernels reported."""
+        _raise_for(_ffi.lib().oxb200_run_wait(self.ctx.handle), self.ctx.last_error())
+
     def clear_bindings(self):
         _raise_for(_ffi.lib().oxb200_clear_bindings(self.ctx.handle), self.ctx.last_error())
 
     # ---- measurement helpers: the same run split into stage / resident launches / read ----
     def upload(self, feeds):
-        lanes = _lanes(feeds, self.graph.input_names)
+        lanes = _lanes(feeds, self.graph.input_names, self._input_types)
         with self._lock:
             self.ensure_planned(feeds)
             io = self._call_io()
