@@ -53,6 +53,8 @@ struct PagedAttention {
 };
 size_t paged_attention_workspace(const PagedAttention& a);
 void paged_attention(const PagedAttention& a, cudaStream_t s);
+// Its sequences of at least `least_rows` packed rows (new rows times query heads of a key head).
+void paged_attention_prompts(const PagedAttention& a, int least_rows, cudaStream_t s);
 
 // y[m][n] = sum_k x[m][k] * (code[n][k] - zero[n][k / group]) * scale[n][k / group] + bias[n]
 struct Linear4 {

@@ -34,6 +34,7 @@ struct Shape {
   static constexpr size_t kSmem = (size_t)kWarps * kRing;
   static_assert(kSmem >= (size_t)kWarps * kRows * KD * 4, "the warps' accumulators meet where the ring was");
 };
+constexpr int kShortRows = 64;  // packed rows of a sequence up to which it is streamed
 constexpr int kMinTiles = 2;  // tiles that a block takes at least: below, joining the parts costs more than the keys
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -399,9 +400,13 @@ size_t paged_attention_workspace(const PagedAttention& a) {
 
 void paged_attention(const PagedAttention& a, cudaStream_t s) {
   if (a.t.tokens == 0) return;
-  const int most_rows = 0x7fffffff;
+  const int group = a.heads / a.kv_heads;
+  const bool products = a.size <= 128;  // a wider head's tiles do not fit tensor memory: the streaming kernel takes all rows
+  const int most_rows = products ? kShortRows : 0x7fffffff;
   if (a.dt == DT::F16) launch_short<__half>(a, most_rows, s);
   else launch_short<__nv_bfloat16>(a, most_rows, s);
+  const int64_t longest = a.max_query > 0 ? a.max_query : a.t.tokens;
+  if (products && longest * group > kShortRows) paged_attention_prompts(a, kShortRows + 1, s);
 }
 
 }  // namespace k
