@@ -26,7 +26,7 @@ namespace k {
 namespace umma {
 
 constexpr int PR_KEYS = 128, PR_ROWS = 128;
-constexpr int PR_THREADS = 320;
+constexpr int PR_THREADS = 384;  // three warpgroups; the last two warps of the third idle
 constexpr float PR_GROWTH = 8.f;  // log2 of how far probabilities may exceed 1 before the output is rescaled
 
 template <int KD>
@@ -173,6 +173,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
   const int tail0 = q.length % p.box == 0 ? 0 : q.length - (most - 1) * PR_KEYS, tail1 = (tail0 + p.box - 1) / p.box * p.box;
   const bool tail = most > 0 && most * PR_KEYS > q.length && q.length % p.box != 0;
 
+  // 168 registers a thread at the launch, 64512 together: 216 for the rows' warpgroups and 72 for the third are 64512 again
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   if (warp == 9) {
     // ---------------- keys and values ----------------
     const int boxes = PR_KEYS / p.box;
@@ -272,8 +275,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
       }
     }
     __syncwarp();
+  }
   } else {
     // ---------------- rows ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int t = warp >> 2, quarter = warp & 3, first_row = row0 + t * PR_ROWS;
     {  // the tile's queries, as TMA would have laid them out: 16 bytes c of a row lie at c ^ (row & 7)
       uint8_t* const dst = base_ptr + q_off + t * S::kTile;
@@ -295,6 +300,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
     const int limit = row < rows ? max(0, q.length - q.rows + row / group + 1) : 0;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_col = tmem + lane_base + S::kScores + t * 128, o_col = tmem + lane_base + S::kOut + t * KD;
+    const uint64_t slope2 = both(p.slope);
     float top = -INFINITY, sum = 0.f;  // the maximum that the output is relative to, and the sum
     bool whole = true;
     for (int j = 0; j < nt[t]; ++j) {
@@ -344,19 +350,24 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
         }
       }
       const float bias = top == -INFINITY ? 0.f : top * p.slope;
-      float part[2] = {0.f, 0.f};
+      uint64_t part = 0;  // two sums
+      const uint64_t bias2 = both(-bias);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float x = ex2(fmaf(__uint_as_float(r[c][2 * i]), p.slope, -bias)), y = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), p.slope, -bias));
-          part[0] += x, part[1] += y;
+          float x, y;
+          unpack2(fmap(pack2(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), slope2, bias2), x, y);
+          x = ex2(x), y = ex2(y);
+          part = addp(part, pack2(x, y));
           w[i] = pack_pair(x, y, (T*)nullptr);
         }
         tmem_st16(s_col + 16 * c, w);
       }
-      sum += part[0] + part[1];
+      float even, odd;
+      unpack2(part, even, odd);
+      sum += even + odd;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
