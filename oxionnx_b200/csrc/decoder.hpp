@@ -53,8 +53,11 @@ struct PagedAttention {
 };
 size_t paged_attention_workspace(const PagedAttention& a);
 void paged_attention(const PagedAttention& a, cudaStream_t s);
-// Its sequences of at least `least_rows` packed rows (new rows times query heads of a key head).
-void paged_attention_prompts(const PagedAttention& a, int least_rows, cudaStream_t s);
+// Its sequences of at least `least_rows` packed rows (new rows times query heads of a key head), on tcgen05.
+bool paged_attention_prompts_fit(const PagedAttention& a);
+size_t paged_attention_prompts_workspace(const PagedAttention& a);
+void paged_attention_prompts(const PagedAttention& a, int least_rows, void* workspace, cudaStream_t s);
+int device_sms();
 
 // y[m][n] = sum_k x[m][k] * (code[n][k] - zero[n][k / group]) * scale[n][k / group] + bias[n]
 struct Linear4 {

@@ -356,15 +356,6 @@ paged_attention_short(PagedAttention a, int most_rows, int min_tiles, float slop
   }
 }
 
-int device_sms() {
-  static const int sms = [] {
-    int n = 0, device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) (void)cudaGetLastError();
-    return n > 0 ? n : 148;
-  }();
-  return sms;
-}
-
 template <typename T, int KD>
 void launch_short(const PagedAttention& a, int most_rows, cudaStream_t s) {
   const size_t smem = Shape<KD>::kSmem + (size_t)a.t.sequences * sizeof(long long);
@@ -391,22 +382,38 @@ void launch_short(const PagedAttention& a, int most_rows, cudaStream_t s) {
   else launch_short<T, 256>(a, most_rows, s);
 }
 
+size_t short_workspace(const PagedAttention& a) {
+  const size_t floats = a.size <= 64 ? Shape<64>::kPart : a.size <= 128 ? Shape<128>::kPart : Shape<256>::kPart;
+  return align_up((size_t)device_sms() * (2 * floats * sizeof(float) + sizeof(int)), 256);
+}
+
+// Is there a call in which some sequence has more than kShortRows packed rows and tcgen05 takes those?
+bool has_prompts(const PagedAttention& a) {
+  const int64_t longest = a.max_query > 0 ? a.max_query : a.t.tokens;
+  return longest * (a.heads / a.kv_heads) > kShortRows && paged_attention_prompts_fit(a);
+}
+
 }  // namespace
 
-size_t paged_attention_workspace(const PagedAttention& a) {
-  const size_t floats = a.size <= 64 ? Shape<64>::kPart : a.size <= 128 ? Shape<128>::kPart : Shape<256>::kPart;
-  return (size_t)device_sms() * (2 * floats * sizeof(float) + sizeof(int));
+int device_sms() {
+  static const int sms = [] {
+    int n = 0, device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) (void)cudaGetLastError();
+    return n > 0 ? n : 148;
+  }();
+  return sms;
 }
+
+size_t paged_attention_workspace(const PagedAttention& a) { return short_workspace(a) + (has_prompts(a) ? paged_attention_prompts_workspace(a) : 0); }
 
 void paged_attention(const PagedAttention& a, cudaStream_t s) {
   if (a.t.tokens == 0) return;
-  const int group = a.heads / a.kv_heads;
-  const bool products = a.size <= 128;  // a wider head's tiles do not fit tensor memory: the streaming kernel takes all rows
-  const int most_rows = products ? kShortRows : 0x7fffffff;
+  const bool prompts = has_prompts(a);
+  // a head that is too wide for tensor memory, or has more query heads than a tile has rows: the streaming kernel takes all rows
+  const int most_rows = prompts || paged_attention_prompts_fit(a) ? kShortRows : 0x7fffffff;
   if (a.dt == DT::F16) launch_short<__half>(a, most_rows, s);
   else launch_short<__nv_bfloat16>(a, most_rows, s);
-  const int64_t longest = a.max_query > 0 ? a.max_query : a.t.tokens;
-  if (products && longest * group > kShortRows) paged_attention_prompts(a, kShortRows + 1, s);
+  if (prompts) paged_attention_prompts(a, kShortRows + 1, (uint8_t*)a.workspace + short_workspace(a), s);
 }
 
 }  // namespace k
