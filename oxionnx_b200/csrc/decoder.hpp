@@ -63,15 +63,44 @@ int device_sms();
 struct Linear4 {
   const void* x;
   void* y;
-  const uint8_t* codes;
-  const float* scales;
+  // laid out as Linear4Layout has them
+  const void* codes;
+  const void* scales;
   const uint8_t* zeros;   // null: 8
+  bool scales_f16;        // scales are f16, f32 otherwise
   const float* bias;      // null: none
   int64_t rows;
   int k, n, group, groups;  // groups: of one output's inputs, the last one perhaps short
   DT dt;                    // x and y
 };
 void linear4(const Linear4& a, cudaStream_t s);
+
+// Where codes, scales and zero points of an [n][k] matrix lie on the device.  Outputs come in tiles of 16 (the last one filled
+// up with outputs of scale 0), inputs in blocks of 64 (filled up with any code: x is 0 there).  A block of a tile is 512 bytes,
+// 16 for each lane of a warp: lane (g, q) = (lane / 4, lane % 4) has four inputs of every 16, 4 q on, of the outputs g and g + 8;
+// a word holds those of 32 inputs, the even ones in nibbles 0-3 and the odd ones in 4-7.  So a group of 16 is one fragment's.  Scales and zero points (a byte each) of a tile
+// and a group lie side by side, output g at 2 g and output g + 8 at 2 g + 1.
+struct Linear4Layout {
+  static int64_t tiles(int64_t n) { return (n + 15) / 16; }
+  static int64_t code_bytes(int64_t n, int64_t k) { return tiles(n) * ((k + 63) / 64) * 512; }
+  static int64_t of_group(int64_t n, int64_t group, int64_t groups) { return (n / 16 * groups + group) * 16 + n % 8 * 2 + n % 16 / 8; }
+  // packed[n][groups][group / 2]: two codes a byte, the even one low
+  static void codes(const float* packed, int64_t n, int64_t k, int64_t group, uint8_t* out) {
+    const int64_t blocks = (k + 63) / 64, row_bytes = (k + group - 1) / group * (group / 2);
+    uint32_t* const words = (uint32_t*)out;
+    for (int64_t o = 0; o < n; ++o)
+      for (int64_t w = 0; w < blocks * 8; ++w) {  // word (w % 2) of lane q = w / 2 % 4 in block w / 8
+        const int64_t q = w / 2 % 4;
+        uint32_t v = 0;
+        for (int64_t j = 0; j < 4; ++j) {  // two inputs each
+          const int64_t at = w / 8 * 32 + w % 2 * 16 + j / 2 * 8 + q * 2 + j % 2;
+          const uint32_t byte = at < row_bytes ? (uint32_t)packed[o * row_bytes + at] : 0u;
+          v |= (byte & 15u) << (4 * j) | (byte >> 4) << (16 + 4 * j);
+        }
+        words[((o / 16 * blocks + w / 8) * 32 + o % 8 * 4 + q) * 4 + o % 16 / 8 * 2 + w % 2] = v;
+      }
+  }
+};
 
 }  // namespace k
 }  // namespace oxb

@@ -16,6 +16,8 @@
 #include <limits>
 #include <memory>
 
+#include <cuda_fp16.h>
+
 #include "decoder.hpp"
 #include "runtime.hpp"
 
@@ -3114,26 +3116,40 @@ void Planner::plan_matmul_4bit(const NodeDef& n) {
   a.rows = prod(xv.shape) / K;
   a.k = (int)K, a.n = (int)N, a.group = (int)group, a.groups = (int)groups;
   a.dt = xv.dt;
-  auto bytes_form = [&](const HostTensor* t, const std::string& of) {
-    return (uint8_t*)C.resident_form(of, "bytes", std::max<size_t>(t->data.size(), 16), [t](void* p) {
-      for (size_t i = 0; i < t->data.size(); ++i) ((uint8_t*)p)[i] = (uint8_t)t->data[i];
-    }, cacheable_const(of));
-  };
-  auto lanes_form = [&](const HostTensor* t, const std::string& of) {
-    return (const float*)C.resident_form(of, "raw_f32", std::max<size_t>(t->data.size() * 4, 4), [t](void* p) { std::memcpy(p, t->data.data(), t->data.size() * 4); },
-                                         cacheable_const(of));
-  };
-  a.codes = bytes_form(codes, in_name(n, 1));
-  a.scales = lanes_form(scales, in_name(n, 2));
-  if (zeros) a.zeros = bytes_form(zeros, in_name(n, 3));
-  if (bias) a.bias = lanes_form(bias, in_name(n, 5));
+  // laid out once for the context, as the kernels take them
+  using Layout4 = k::Linear4Layout;
+  const std::string shape = "linear4 " + std::to_string(N) + "x" + std::to_string(K) + "/" + std::to_string(group);
+  a.codes = C.resident_form(in_name(n, 1), shape, (size_t)Layout4::code_bytes(N, K),
+                            [&](void* p) { Layout4::codes(codes->data.data(), N, K, group, (uint8_t*)p); }, cacheable_const(in_name(n, 1)));
+  // scales keep their 16 bits where f16 holds them, as it does those of a model that stores them so
+  const int64_t lanes = Layout4::tiles(N) * groups * 16;
+  a.scales_f16 = true;
+  for (float v : scales->data) a.scales_f16 = a.scales_f16 && __half2float(__float2half_rn(v)) == v;
+  a.scales = C.resident_form(in_name(n, 2), shape, (size_t)lanes * (a.scales_f16 ? 2 : 4), [&](void* p) {
+    for (int64_t o = 0; o < N; ++o)
+      for (int64_t g = 0; g < groups; ++g) {
+        const float v = scales->data[o * groups + g];
+        if (a.scales_f16) ((__half*)p)[Layout4::of_group(o, g, groups)] = __float2half_rn(v);
+        else ((float*)p)[Layout4::of_group(o, g, groups)] = v;
+      }
+  }, cacheable_const(in_name(n, 2)));
+  if (zeros)
+    a.zeros = (const uint8_t*)C.resident_form(in_name(n, 3), shape, (size_t)lanes, [&](void* p) {
+      for (int64_t o = 0; o < N; ++o)
+        for (int64_t g = 0; g < groups; ++g) {
+          const int byte = (int)zeros->data[o * ceil_div(groups, 2) + g / 2];
+          ((uint8_t*)p)[Layout4::of_group(o, g, groups)] = (uint8_t)(g & 1 ? byte >> 4 : byte & 15);
+        }
+    }, cacheable_const(in_name(n, 3)));
+  if (bias)
+    a.bias = (const float*)C.resident_form(in_name(n, 5), "raw_f32", (size_t)N * 4, [&](void* p) { std::memcpy(p, bias->data.data(), (size_t)N * 4); }, cacheable_const(in_name(n, 5)));
 
   const int yi = add_typed(n.outputs[0], os, xv.dt);
   V(yi).late_address = true;
   Step& st = add_step(n, "linear4", 1, {xi}, {yi});
   st.work = 2.0 * (double)a.rows * (double)K * (double)N;
   st.work_is_bytes = false;
-  st.param_bytes = (double)codes->data.size() + 4.0 * (double)scales->data.size() + (zeros ? (double)zeros->data.size() : 0.0);
+  st.param_bytes = (double)Layout4::code_bytes(N, K) + (double)lanes * ((a.scales_f16 ? 2 : 4) + (zeros ? 1 : 0)) + (bias ? 4.0 * (double)N : 0.0);
   st.launch = [this, a, xi, yi](cudaStream_t s) {
     k::Linear4 b = a;
     b.x = V(xi).ptr;
