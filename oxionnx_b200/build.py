@@ -24,14 +24,14 @@ KERNEL = [f for f in COMMON if f != "--fmad=false"]
 OBJECTS = {
     "kernels_glue": ("kernels_glue.cu", COMMON),
     **{name: (name + ".cu", KERNEL) for name in ("kernels_simt", "kernels_umma", "umma_i8", "umma_tf32", "umma_f16", "umma_small_i8", "umma_small_float",
-                                                  "umma_probe", "umma_chain", "umma_attention", "paged_append", "paged_attention", "umma_prompt", "linear4")},
+                                                  "umma_probe", "umma_chain", "umma_attention", "paged_append", "paged_attention", "umma_prompt", "linear4", "umma_linear4")},
     **{f"umma_i8_{tile}": ("umma_i8_tile.cu", KERNEL + [f"-DOXB_TILE={bn}", f"-DOXB_PAIR={pair}"])
        for tile, bn, pair in (("32", 32, "false"), ("64", 64, "false"), ("128", 128, "false"), ("256", 256, "false"), ("pair", 256, "true"))},
     **{name: (name + ".cpp", COMMON) for name in ("runtime", "planner", "abi", "onnx_model", "model_abi")},
 }
 # headers of the decoder operators, which nothing but these objects includes
 DECODER_HEADERS = ["decoder.hpp", "decoder_device.cuh", "decoder_schedule.hpp"]
-DECODER_OBJECTS = ("planner", "paged_append", "paged_attention", "umma_prompt", "linear4")
+DECODER_OBJECTS = ("planner", "paged_append", "paged_attention", "umma_prompt", "linear4", "umma_linear4")
 HEADERS = ["common.hpp", "kernels.hpp", "runtime.hpp", "umma_kernel.cuh", "umma_epilogue8.cuh", "umma_launch.cuh", "umma_small.cuh", "pdl.cuh", "umma_chain.cuh", "model.hpp", "abi_internal.hpp", os.path.join("..", "..", "include", "oxb200.h")]
 
 

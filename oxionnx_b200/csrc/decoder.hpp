@@ -72,16 +72,21 @@ struct Linear4 {
   int64_t rows;
   int k, n, group, groups;  // groups: of one output's inputs, the last one perhaps short
   DT dt;                    // x and y
+  void* workspace;          // linear4_workspace bytes, or null
+  int* err;
 };
+size_t linear4_workspace(const Linear4& a);
 void linear4(const Linear4& a, cudaStream_t s);
+bool linear4_many_rows(const Linear4& a);
+void linear4_prompt(const Linear4& a, cudaStream_t s);  // many rows of 16 bits
 
-// Where codes, scales and zero points of an [n][k] matrix lie on the device.  Outputs come in tiles of 16 (the last one filled
+// Where codes, scales and zero points of an [n][k] matrix lie on the device.  Outputs come in tiles of 16 (the last ones filled
 // up with outputs of scale 0), inputs in blocks of 64 (filled up with any code: x is 0 there).  A block of a tile is 512 bytes,
 // 16 for each lane of a warp: lane (g, q) = (lane / 4, lane % 4) has four inputs of every 16, 4 q on, of the outputs g and g + 8;
 // a word holds those of 32 inputs, the even ones in nibbles 0-3 and the odd ones in 4-7.  So a group of 16 is one fragment's.  Scales and zero points (a byte each) of a tile
 // and a group lie side by side, output g at 2 g and output g + 8 at 2 g + 1.
 struct Linear4Layout {
-  static int64_t tiles(int64_t n) { return (n + 15) / 16; }
+  static int64_t tiles(int64_t n) { return (n + 63) / 64 * 4; }  // whole runs of four: no kernel has to look where they end
   static int64_t code_bytes(int64_t n, int64_t k) { return tiles(n) * ((k + 63) / 64) * 512; }
   static int64_t of_group(int64_t n, int64_t group, int64_t groups) { return (n / 16 * groups + group) * 16 + n % 8 * 2 + n % 16 / 8; }
   // packed[n][groups][group / 2]: two codes a byte, the even one low

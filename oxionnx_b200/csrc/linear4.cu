@@ -9,6 +9,8 @@
 // as the sum of three bf16 numbers (8 bits of the significand each, all 24 of them), whose products are exact as well.
 //
 // A block has 16 (or 32) outputs and splits the inputs over its warps; the warps' sums meet in shared memory in one order.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "decoder_device.cuh"
@@ -17,6 +19,8 @@ namespace oxb {
 namespace k {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8;
 
@@ -67,9 +71,9 @@ __device__ __forceinline__ uint32_t minus<__nv_bfloat16>(uint32_t a, uint32_t b)
 
 // Four lanes of x from `src` (those from `left` on are zeros) as `SPLIT` numbers each, two to a word.
 template <typename T, int SPLIT>
-__device__ __forceinline__ void load4(const T* src, int left, uint32_t (&w)[SPLIT][8], int at, bool aligned) {
+__device__ __forceinline__ void load4(const T* src, int left, bool whole, uint32_t (&w)[SPLIT][8], int at) {
   if constexpr (sizeof(T) == 2) {
-    if (left >= 4 && aligned) {
+    if (whole) {
       const uint2 a = *(const uint2*)src;
       w[0][at] = a.x, w[0][at + 1] = a.y;
     } else {
@@ -81,7 +85,7 @@ __device__ __forceinline__ void load4(const T* src, int left, uint32_t (&w)[SPLI
     }
   } else {
     float v[4];
-    if (left >= 4 && aligned) {
+    if (whole) {
       *(float4*)v = *(const float4*)src;
     } else {
 #pragma unroll
@@ -103,57 +107,78 @@ __device__ __forceinline__ void load4(const T* src, int left, uint32_t (&w)[SPLI
   }
 }
 
-// MT: tiles of 16 outputs; NT: of 8 rows; SUB: groups of a 64-input block (4, 2 or 1); ST: type of the scales.
-template <typename T, int MT, int NT, int SUB, typename ST>
-__global__ void __launch_bounds__(kWarps * 32) linear4_rows(Linear4 a, int64_t row0) {
+// MT: tiles of 16 outputs; NT: of 8 rows; SUB: groups of a 64-input block (4, 2 or 1); ZP: zero points, 8 without; ST: type of
+// the scales.  `shift`: log2 of the blocks of a group where a group is at least a block.  The blocks of a cluster split the
+// inputs further.
+template <typename T, int MT, int NT, int SUB, bool ZP, typename ST>
+__global__ void __launch_bounds__(kWarps * 32) linear4_rows(Linear4 a, int64_t row0, int shift, int splits) {
   using H = typename Operand<T>::type;
   constexpr int SPLIT = sizeof(T) == 4 ? 3 : 1, STEPS = 4 / SUB;  // k16 steps of a group within the block
-  extern __shared__ float meet[];                                 // [warp][MT * 16 outputs][NT * 8 rows + 1]
-  pdl_enter();
+  constexpr int LD = NT * 8 + 1;
+  __shared__ float meet[kWarps / 2][MT * 16][LD], sums[MT * 16 * NT * 8];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int tile0 = blockIdx.x * MT, tiles = (a.n + 15) / 16, blocks = (a.k + 63) / 64;
+  const int tile0 = blockIdx.x / splits * MT, slice = blockIdx.x % splits * kWarps + warp, blocks = (a.k + 63) / 64;
   row0 += (int64_t)blockIdx.y * NT * 8;
-  const int first = (int)((int64_t)blocks * warp / kWarps), last = (int)((int64_t)blocks * (warp + 1) / kWarps);
+  const int first = (int)((int64_t)blocks * slice / (splits * kWarps)), last = (int)((int64_t)blocks * (slice + 1) / (splits * kWarps));
   const int rows = (int)min((int64_t)NT * 8, a.rows - row0);
   const bool aligned = a.k % 4 == 0 && ((uintptr_t)a.x & 15) == 0;
 
-  float acc[MT][NT][4] = {};
-  const uint4* codes[MT];
-  const ST* scales[MT];
-  const uint8_t* zeros[MT];
+  // addresses: one for the thread block and 32 bits for the lane (the layout fills the last blocks' tiles up)
+  const uint8_t* const codes = (const uint8_t*)a.codes + (int64_t)tile0 * blocks * 512;
+  const uint8_t* const scales = (const uint8_t*)a.scales + (int64_t)tile0 * a.groups * 16 * sizeof(ST);
+  const uint8_t* const zeros = ZP ? a.zeros + (int64_t)tile0 * a.groups * 16 : nullptr;
+  const T* const x_base = (const T*)a.x + row0 * a.k;
+  const uint32_t lane_codes = lane * 16;
+  uint32_t x_at[NT];  // rows behind the last are copies of it: their columns of the products go nowhere
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int64_t tile = min(tile0 + m, tiles - 1);
-    codes[m] = (const uint4*)a.codes + tile * blocks * 32 + lane;
-    scales[m] = (const ST*)a.scales + tile * a.groups * 16 + 2 * g;
-    zeros[m] = a.zeros ? a.zeros + tile * a.groups * 16 + 2 * g : nullptr;
-  }
+  for (int t = 0; t < NT; ++t) x_at[t] = (uint32_t)min(t * 8 + g, rows - 1) * a.k + q * 4;
+
+  float acc[MT][NT][4] = {};
+  // the codes are the session's own: the first of them need not wait for the kernel in front
+  uint4 ahead[MT];
+  if (first < last)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) ahead[m] = __ldcs((const uint4*)(codes + (uint32_t)(m * blocks + first) * 512u + lane_codes));
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
 #pragma unroll 2
   for (int b = first; b < last; ++b) {
+    uint32_t x[NT][SPLIT][8];
+    if (aligned && b * 64 + 64 <= a.k) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load4<T, SPLIT>(x_base + (x_at[t] + (uint32_t)(b * 64 + j * 16)), 4, true, x[t], 2 * j);
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) load4<T, SPLIT>(x_base + (x_at[t] + (uint32_t)(b * 64 + j * 16)), a.k - (b * 64 + j * 16 + q * 4), false, x[t], 2 * j);
+    }
     uint4 w[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) w[m] = __ldcs(codes[m] + (int64_t)b * 32);
-    uint32_t x[NT][SPLIT][8];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int row = t * 8 + g;
-      const bool real = row < rows;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = b * 64 + j * 16 + q * 4;
-        load4<T, SPLIT>((const T*)a.x + (real && k < a.k ? (row0 + row) * a.k + k : 0), real ? a.k - k : 0, x[t], 2 * j, aligned);
-      }
+    for (int m = 0; m < MT; ++m) {
+      w[m] = ahead[m];
+      if (b + 1 < last) ahead[m] = __ldcs((const uint4*)(codes + (uint32_t)(m * blocks + b + 1) * 512u + lane_codes));
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
-        const int group = SUB == 1 ? b * 64 / a.group : min(b * SUB + s, a.groups - 1);  // of a block's groups behind the last, the codes are zeros' and x is 0
-        const ST* const sc = scales[m] + (int64_t)group * 16;
-        const float scale0 = to_f32(sc[0]), scale1 = to_f32(sc[1]);
+        const int group = SUB == 1 ? b >> shift : min(b * SUB + s, a.groups - 1);  // a block's groups behind the last have x of 0
+        const uint32_t of_group = (uint32_t)(m * a.groups + group) * 16u + 2u * g;
+        float scale0, scale1;
+        if constexpr (sizeof(ST) == 2) {
+          const float2 v = __half22float2(*(const __half2*)(scales + of_group * 2u));
+          scale0 = v.x, scale1 = v.y;
+        } else {
+          const float2 v = *(const float2*)(scales + of_group * 4u);
+          scale0 = v.x, scale1 = v.y;
+        }
         uint32_t z0 = kOffset<H> + 0x00080008u, z1 = z0;
-        if (zeros[m]) {
-          const uint32_t both = *(const uint16_t*)(zeros[m] + (int64_t)group * 16);
+        if constexpr (ZP) {
+          const uint32_t both = *(const uint16_t*)(zeros + of_group);
           z0 = kOffset<H> + (both & 15u) * 0x10001u, z1 = kOffset<H> + (both >> 8) * 0x10001u;
         }
         float part[NT][4] = {};
@@ -179,34 +204,74 @@ __global__ void __launch_bounds__(kWarps * 32) linear4_rows(Linear4 a, int64_t r
       }
     }
   }
-  constexpr int LD = NT * 8 + 1;
+
+  // the warps' sums: the upper half's onto the lower half's, then those together
+  auto at = [&](int m, int t, int e) -> float& { return meet[warp % (kWarps / 2)][m * 16 + g + (e >> 1) * 8][t * 8 + q * 2 + (e & 1)]; };
+  if (warp >= kWarps / 2)
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) meet[(warp * MT * 16 + m * 16 + g + (e >> 1) * 8) * LD + t * 8 + q * 2 + (e & 1)] = acc[m][t][e];
+        for (int e = 0; e < 4; ++e) at(m, t, e) = acc[m][t][e];
   __syncthreads();
+  if (warp < kWarps / 2)
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) at(m, t, e) += acc[m][t][e];
+  __syncthreads();
+  auto give = [&](int o, int row, float sum) {
+    const int n = tile0 * 16 + o;
+    if (n < a.n) ((T*)a.y)[(row0 + row) * a.n + n] = from_f32<T>(a.bias ? sum + a.bias[n] : sum);
+  };
   for (int i = threadIdx.x; i < MT * 16 * rows; i += kWarps * 32) {
-    const int o = i % (MT * 16), row = i / (MT * 16), n = tile0 * 16 + o;
-    if (n >= a.n) continue;
+    const int o = i % (MT * 16), row = i / (MT * 16);
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += meet[(w * MT * 16 + o) * LD + row];
-    ((T*)a.y)[(row0 + row) * a.n + n] = from_f32<T>(a.bias ? sum + a.bias[n] : sum);
+    for (int w = 0; w < kWarps / 2; ++w) sum += meet[w][o][row];
+    if (splits == 1) give(o, row, sum);
+    else sums[i] = sum;
+  }
+  if (splits > 1) {  // the cluster's sums, in the order of the inputs
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = threadIdx.x * splits + (int)cluster.block_rank(); i < MT * 16 * rows; i += kWarps * 32 * splits) {
+      float sum = 0.f;
+      for (int c = 0; c < splits; ++c) sum += cluster.map_shared_rank(sums, c)[i];
+      give(i % (MT * 16), i / (MT * 16), sum);
+    }
+    cluster.sync();
   }
 }
 
-template <typename T, int MT, int NT, int SUB, typename ST>
+template <typename T, int MT, int NT, int SUB, bool ZP, typename ST>
 void launch_rows(const Linear4& a, int64_t row0, int64_t rows, cudaStream_t s) {
-  const size_t smem = (size_t)kWarps * MT * 16 * (NT * 8 + 1) * sizeof(float);
-  static_assert((size_t)kWarps * MT * 16 * (NT * 8 + 1) * sizeof(float) <= 48 * 1024, "no opt-in");
-  const dim3 grid((unsigned)ceil_div(ceil_div(a.n, 16), MT), (unsigned)ceil_div(rows, NT * 8));
-  launch(linear4_rows<T, MT, NT, SUB, ST>, grid, dim3(kWarps * 32), smem, s, a, row0);
+  // The inputs are split over as many blocks as bring the grid to two blocks an SM, while a warp keeps two 64-input blocks.
+  const int64_t outputs = ceil_div(ceil_div(a.n, 16), MT), row_blocks = ceil_div(rows, NT * 8), blocks = ceil_div(a.k, 64);
+  int splits = 1, shift = 0;
+  while (splits < 8 && outputs * row_blocks * splits * 2 <= 2 * device_sms() && blocks >= 2LL * kWarps * splits * 2) splits *= 2;
+  while ((64 << shift) < a.group) ++shift;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(outputs * splits), (unsigned)row_blocks);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 2 : 1;
+  OXB_CUDA(cudaLaunchKernelEx(&cfg, linear4_rows<T, MT, NT, SUB, ZP, ST>, a, row0, shift, splits));
 }
 template <typename T, int MT, int NT, int SUB>
 void launch_rows(const Linear4& a, int64_t row0, int64_t rows, cudaStream_t s) {
-  a.scales_f16 ? launch_rows<T, MT, NT, SUB, __half>(a, row0, rows, s) : launch_rows<T, MT, NT, SUB, float>(a, row0, rows, s);
+  if (a.scales_f16) a.zeros ? launch_rows<T, MT, NT, SUB, true, __half>(a, row0, rows, s) : launch_rows<T, MT, NT, SUB, false, __half>(a, row0, rows, s);
+  else a.zeros ? launch_rows<T, MT, NT, SUB, true, float>(a, row0, rows, s) : launch_rows<T, MT, NT, SUB, false, float>(a, row0, rows, s);
 }
 template <typename T, int MT, int NT>
 void launch_rows(const Linear4& a, int64_t row0, int64_t rows, cudaStream_t s) {
@@ -216,20 +281,31 @@ void launch_rows(const Linear4& a, int64_t row0, int64_t rows, cudaStream_t s) {
 }
 template <typename T>
 void launch_rows(const Linear4& a, cudaStream_t s) {
+  // Tiles of 16 outputs for a warp, in us at rows x K x N, 1 / 2 / 4 tiles: 1 x 4096 x 16384 17.9 / 13.4 / 12.5, 8 x 4096 x 4096
+  // 10.9 / 8.9 / 6.4, 16 x 4096 x 4096 10.8 / 10.1 / 8.5, where rows are fetched once for all of them; small matrices want the
+  // blocks: 1 x 1024 x 1024 2.3 / 2.5 / 3.0, 5 x 1000 x 1111 (f32) 3.6 / 3.9 / 4.5; and so do 32 rows, whose fragments fill the
+  // registers: 32 x 4096 x 4096 12.9 / 16.2 / 18.2.
+  const bool large = (int64_t)a.n * a.k >= 148LL * 65536;
   // grid.y holds 65535 blocks of rows
   for (int64_t row0 = 0; row0 < a.rows; row0 += 65535LL * 16) {
     const int64_t rows = std::min<int64_t>(a.rows - row0, 65535LL * 16);
-    if (rows <= 8) launch_rows<T, 1, 1>(a, row0, rows, s);
-    else if (rows <= 16 || sizeof(T) == 4) launch_rows<T, 2, 2>(a, row0, rows, s);
-    else launch_rows<T, 2, 4>(a, row0, rows, s);
+    if (rows <= 8) large ? launch_rows<T, 4, 1>(a, row0, rows, s) : launch_rows<T, 1, 1>(a, row0, rows, s);
+    else if (rows <= 16 || sizeof(T) == 4) large ? launch_rows<T, 4, 2>(a, row0, rows, s) : launch_rows<T, 1, 2>(a, row0, rows, s);
+    else launch_rows<T, 1, 4>(a, row0, rows, s);
   }
 }
 
 }  // namespace
 
+// 16-bit rows from here on run on tcgen05 (umma_linear4.cu), whose block takes 128 outputs by up to 256 rows.
+constexpr int64_t kManyRows = 33;
+
+bool linear4_many_rows(const Linear4& a) { return a.dt != DT::F32 && a.rows >= kManyRows; }
+
 void linear4(const Linear4& a, cudaStream_t s) {
   if (a.rows == 0) return;
-  if (a.dt == DT::F32) launch_rows<float>(a, s);
+  if (linear4_many_rows(a)) linear4_prompt(a, s);
+  else if (a.dt == DT::F32) launch_rows<float>(a, s);
   else if (a.dt == DT::F16) launch_rows<__half>(a, s);
   else launch_rows<__nv_bfloat16>(a, s);
 }

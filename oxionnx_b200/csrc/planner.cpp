@@ -3144,18 +3144,22 @@ void Planner::plan_matmul_4bit(const NodeDef& n) {
   if (bias)
     a.bias = (const float*)C.resident_form(in_name(n, 5), "raw_f32", (size_t)N * 4, [&](void* p) { std::memcpy(p, bias->data.data(), (size_t)N * 4); }, cacheable_const(in_name(n, 5)));
 
+  a.err = S.err_flag_;
+  if (const size_t bytes = k::linear4_workspace(a)) a.workspace = owned_buffer(bytes);
+  const bool many = k::linear4_many_rows(a);
   const int yi = add_typed(n.outputs[0], os, xv.dt);
   V(yi).late_address = true;
-  Step& st = add_step(n, "linear4", 1, {xi}, {yi});
+  Step& st = add_step(n, many ? "umma_linear4" : "linear4", many ? 0 : 1, {xi}, {yi});
+  st.late_address = many;
   st.work = 2.0 * (double)a.rows * (double)K * (double)N;
   st.work_is_bytes = false;
   st.param_bytes = (double)Layout4::code_bytes(N, K) + (double)lanes * ((a.scales_f16 ? 2 : 4) + (zeros ? 1 : 0)) + (bias ? 4.0 * (double)N : 0.0);
-  st.launch = [this, a, xi, yi](cudaStream_t s) {
+  st.launch = [this, a, xi, yi, many](cudaStream_t s) {
     k::Linear4 b = a;
     b.x = V(xi).ptr;
     b.y = V(yi).ptr;
     k::linear4(b, s);
-    C.counters.simt_launches++;
+    (many ? C.counters.umma_launches : C.counters.simt_launches)++;
     C.counters.kernel_launches++;
   };
   widen(n, n.outputs[0]);

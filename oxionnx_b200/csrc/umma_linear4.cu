@@ -1,0 +1,342 @@
+// Many 16-bit rows times a matrix of 4-bit codes, on tcgen05: the matrix stays in 4 bits in memory and becomes 16-bit lanes on
+// its way into the products.
+//
+// A block has 128 outputs and up to 256 rows of x.  Outputs are the rows of the accumulator, so that a weight is an element of
+// the A operand, which tensor memory may hold: the thread of an output decodes 64 of its codes, (code - zero) * scale rounded
+// once to x's type, and writes them there, a store of 32 columns and no shared memory.  x comes through TMA as the B operand.
+// Eight warps decode (four a block of 64 inputs, in turns), one thread brings x, one issues the products.  The products of a
+// block of 64 inputs by 256 rows take 512 cycles, the decoding of its 128 x 64 codes about half of that of each scheduler.
+//
+// The roundings of the weights are as large as those of the result (half a step of x's type each, and independent).
+// Every wait is bounded.
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "decoder_device.cuh"
+#include "umma_kernel.cuh"
+
+namespace oxb {
+namespace k {
+
+namespace umma {
+
+constexpr int L4_OUTPUTS = 128, L4_K = 64;
+constexpr int L4_THREADS = 320;
+constexpr int L4_WEIGHT_STAGES = 4;  // 32 columns of tensor memory each
+
+template <int ROWS>
+struct Linear4Shape {
+  static constexpr uint32_t kTile = ROWS * 128u;  // rows of 64 lanes
+  static constexpr int kStages = ROWS == 256 ? 6 : 8;
+  static constexpr uint32_t kSmem = kStages * kTile + 1024u;
+  static constexpr uint32_t kAcc = 0, kWeights = 256;  // columns of tensor memory
+  static_assert(kStages * kTile >= 2 * 8192, "the rows leave where x was");
+};
+
+struct alignas(64) Linear4Params {
+  CUtensorMap x;
+  Linear4 a;
+  int blocks, shift;  // of 64 inputs; log2 of the inputs of a group
+  uint32_t idesc;
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t code_bits, uint32_t zero, float scale);
+// 1024 + code is exact in f16, so is code - zero; one product, one rounding (the scale is exact in f32)
+template <>
+__device__ __forceinline__ uint32_t decode_pair<__half>(uint32_t bits, uint32_t zero, float scale) {
+  const uint32_t v = bits | 0x64006400u;
+  const float2 d = __half22float2(__hsub2(*(const __half2*)&v, *(const __half2*)&zero));
+  const __half2 r = __floats2half2_rn(d.x * scale, d.y * scale);
+  return *(const uint32_t*)&r;
+}
+template <>
+__device__ __forceinline__ uint32_t decode_pair<__nv_bfloat16>(uint32_t bits, uint32_t zero, float scale) {
+  const uint32_t v = bits | 0x43004300u;
+  const __nv_bfloat162 d = __hsub2(*(const __nv_bfloat162*)&v, *(const __nv_bfloat162*)&zero);
+  const uint32_t w = *(const uint32_t*)&d;
+  const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w << 16) * scale, __uint_as_float(w & 0xffff0000u) * scale);
+  return *(const uint32_t*)&r;
+}
+
+__device__ __forceinline__ void l4_mma(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc),
+               "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void l4_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+template <typename T, int ROWS, typename ST>
+__global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __grid_constant__ Linear4Params p) {
+  using S = Linear4Shape<ROWS>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_x_full[S::kStages], bar_x_empty[S::kStages], bar_w_full[L4_WEIGHT_STAGES], bar_w_empty[L4_WEIGHT_STAGES], bar_acc;
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+  const Linear4& a = p.a;
+  const int warp = (int)(threadIdx.x >> 5), lane = (int)(threadIdx.x & 31);
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  volatile int* const abortp = &abort_flag;
+  const int out_blocks = (a.n + L4_OUTPUTS - 1) / L4_OUTPUTS;
+  const int out0 = (int)(blockIdx.x % out_blocks) * L4_OUTPUTS;
+  const int64_t row0 = (int64_t)(blockIdx.x / out_blocks) * ROWS;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < S::kStages; ++i) mbar_init(smem_u32(&bar_x_full[i]), 1), mbar_init(smem_u32(&bar_x_empty[i]), 1);
+    for (int i = 0; i < L4_WEIGHT_STAGES; ++i) mbar_init(smem_u32(&bar_w_full[i]), 4), mbar_init(smem_u32(&bar_w_empty[i]), 1);
+    mbar_init(smem_u32(&bar_acc), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_slot;
+  pdl_enter();
+  auto give_up = [&](int code) {
+    if (!*abortp) {
+      *abortp = 1;
+      atomicExch(a.err, code);
+    }
+  };
+
+  if (warp == 9) {
+    // ---------------- rows of x ----------------
+    if (elect_one()) {
+      for (int b = 0; b < p.blocks; ++b) {
+        const int stage = b % S::kStages;
+        if (b >= S::kStages && !mbar_wait(smem_u32(&bar_x_empty[stage]), ((b / S::kStages) & 1u) ^ 1u, abortp)) {
+          give_up(61);
+          break;
+        }
+        mbar_expect_tx(smem_u32(&bar_x_full[stage]), S::kTile);
+        tma_load_2d(base + stage * S::kTile, &p.x, smem_u32(&bar_x_full[stage]), b * L4_K, (int)row0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ---------------- products ----------------
+    if (elect_one()) {
+      const uint64_t x_at = make_smem_desc(base, 128);
+      const uint32_t w_at = tmem + S::kWeights, acc = tmem + S::kAcc, idesc = p.idesc;
+      bool ok = true;
+      for (int b = 0; b < p.blocks; ++b) {
+        const int stage = b % S::kStages, ws = b % L4_WEIGHT_STAGES;
+        ok = mbar_wait(smem_u32(&bar_x_full[stage]), (b / S::kStages) & 1u, abortp) && mbar_wait(smem_u32(&bar_w_full[ws]), (b / L4_WEIGHT_STAGES) & 1u, abortp);
+        if (!ok) {
+          give_up(62);
+          break;
+        }
+        tc_fence_after();
+        const uint64_t at = x_at + (uint32_t)stage * (S::kTile >> 4);
+#pragma unroll
+        for (int k = 0; k < L4_K / 16; ++k) l4_mma(acc, w_at + ws * 32 + k * 8, at + 2 * k, idesc, k > 0 ? 1u : (b > 0 ? 1u : 0u));
+        tc_commit<false>(smem_u32(&bar_x_empty[stage]));
+        tc_commit<false>(smem_u32(&bar_w_empty[ws]));
+      }
+      if (ok) tc_commit<false>(smem_u32(&bar_acc));
+    }
+    __syncwarp();
+  } else {
+    // ---------------- weights, then the rows' way out ----------------
+    const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int tiles = (a.n + 63) / 64 * 4, tile = min((out0 + r) / 16, tiles - 1), in_tile = r % 8 * 2 + r % 16 / 8;
+    const uint8_t* const codes = (const uint8_t*)a.codes + (int64_t)tile * p.blocks * 512 + r % 8 * 64 + r % 16 / 8 * 8;
+    const ST* const scales = (const ST*)a.scales + (int64_t)tile * a.groups * 16 + in_tile;
+    const uint8_t* const zeros = a.zeros ? a.zeros + (int64_t)tile * a.groups * 16 + in_tile : nullptr;
+    constexpr uint32_t kOffset = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u;
+    uint2 next[4];
+    auto fetch = [&](int b) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) next[q] = *(const uint2*)(codes + (int64_t)b * 512 + q * 16);
+    };
+    if (half < p.blocks) fetch(half);
+    bool ok = true;
+    for (int b = half; b < p.blocks; b += 2) {
+      uint2 now[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) now[q] = next[q];
+      if (b + 2 < p.blocks) fetch(b + 2);
+      // groups of the block's four 16 inputs; those behind the last group meet x of 0
+      float scale[4];
+      uint32_t zero[4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int group = min((b * 64 + s * 16) >> p.shift, a.groups - 1);
+        scale[s] = to_f32(scales[(int64_t)group * 16]);
+        zero[s] = kOffset + (zeros ? zeros[(int64_t)group * 16] : 8u) * 0x10001u;
+      }
+      const int ws = b % L4_WEIGHT_STAGES;
+      if (b >= L4_WEIGHT_STAGES && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_w_empty[ws]), ((b / L4_WEIGHT_STAGES) & 1u) ^ 1u, abortp))) {
+        if (lane == 0) give_up(63);
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t word = h ? now[q].y : now[q].x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)  // inputs 32 h + 16 (e / 2) + 4 q + 2 (e % 2) and the next
+            w[16 * h + 8 * (e / 2) + 2 * q + e % 2] = decode_pair<T>(word >> (4 * e) & 0x000f000fu, zero[2 * h + e / 2], scale[2 * h + e / 2]);
+        }
+      l4_store32(tmem + lane_base + S::kWeights + ws * 32, w);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_w_full[ws]));
+    }
+    if (ok && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_acc), 0u, abortp))) {
+      if (lane == 0) give_up(64);
+      ok = false;
+    }
+    // the four warps of a half go on together or not at all
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+    if (!*abortp) {
+      tc_fence_after();
+      const int out = out0 + r;
+      const float bias = a.bias && out < a.n ? a.bias[out] : 0.f;
+      uint8_t* const staging = base_ptr + half * 8192;  // 32 rows of 128 outputs
+      const int outs = min(L4_OUTPUTS, a.n - out0);
+      const bool wide = a.n % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
+#pragma unroll 1
+      for (int c = 0; c < ROWS / 64; ++c) {
+        const int first = half * (ROWS / 2) + c * 32;
+        uint32_t v[32];
+        tmem_ld32_nowait(tmem + lane_base + S::kAcc + first, v);
+        tmem_ld_wait_for(v);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) *(T*)(staging + e * 256 + r * 2) = from_f32<T>(__uint_as_float(v[e]) + bias);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        const int i = (int)threadIdx.x & 127;
+        if (wide) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int row = e * 8 + i / 16, col = i % 16 * 8;
+            if (row0 + first + row < a.rows && col < outs) *(uint4*)((T*)a.y + (row0 + first + row) * a.n + out0 + col) = *(const uint4*)(staging + row * 256 + col * 2);
+          }
+        } else if (i < outs) {
+#pragma unroll 4
+          for (int row = 0; row < 32; ++row)
+            if (row0 + first + row < a.rows) ((T*)a.y)[(row0 + first + row) * a.n + out0 + i] = *(const T*)(staging + row * 256 + i * 2);
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+      }
+    }
+  }
+
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (abort_flag && threadIdx.x == 0) {
+    // give copies that may still be in flight time to land before the block's shared memory goes away
+    const long long start = clock64();
+    while (clock64() - start < 2000000LL) {
+    }
+  }
+  __syncthreads();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_slot), "r"(512) : "memory");
+}
+
+// Rows of odd length, or at an odd address, once more with a stride that TMA takes.
+__global__ void __launch_bounds__(256) linear4_pad_rows(const uint16_t* x, uint16_t* padded, int64_t rows, int k, int stride) {
+  pdl_enter();
+  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < rows * stride; i += gridDim.x * 256LL) {
+    const int64_t row = i / stride;
+    const int col = (int)(i - row * stride);
+    padded[i] = col < k ? x[row * k + col] : (uint16_t)0;
+  }
+}
+
+}  // namespace umma
+
+using namespace umma;
+
+namespace {
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn tiled_encoder() {
+  static std::once_flag once;
+  static EncodeTiledFn fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &qr) == cudaSuccess && qr == cudaDriverEntryPointSuccess) fn = (EncodeTiledFn)f;
+    (void)cudaGetLastError();
+  });
+  return fn;
+}
+
+template <typename T, int ROWS, typename ST>
+void launch_prompt(const Linear4& a, cudaStream_t s) {
+  using S = Linear4Shape<ROWS>;
+  static std::mutex mu;
+  static bool have[64] = {};
+  int device = 0;
+  OXB_CUDA(cudaGetDevice(&device));
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (device < 0 || device >= 64 || !have[device]) {
+      OXB_CUDA(cudaFuncSetAttribute(umma_linear4_kernel<T, ROWS, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+      if (device >= 0 && device < 64) have[device] = true;
+    }
+  }
+  Linear4Params p{};
+  p.a = a;
+  p.blocks = (a.k + L4_K - 1) / L4_K;
+  while ((1 << p.shift) < a.group) ++p.shift;
+  const void* x = a.x;
+  int64_t stride = a.k;
+  if (a.workspace) {
+    stride = (a.k + 7) / 8 * 8;
+    launch(linear4_pad_rows, dim3((unsigned)std::min<int64_t>(ceil_div(a.rows * stride, 256), 148 * 8)), dim3(256), 0, s, (const uint16_t*)a.x, (uint16_t*)a.workspace, a.rows, a.k, (int)stride);
+    x = a.workspace;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t box[2] = {L4_K, ROWS}, steps[2] = {1, 1};
+  EncodeTiledFn encode = tiled_encoder();
+  if (!encode || encode(&p.x, a.dt == DT::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    OXB_FAIL("MatMulNBits: the driver refused the tensor map of x");
+  // kind::f16: f32 accumulator, A (from tensor memory) and B in x's type, both K-major, 128 x ROWS
+  const uint32_t type = a.dt == DT::F16 ? 0u : 1u;
+  p.idesc = (1u << 4) | (type << 7) | (type << 10) | (((uint32_t)ROWS >> 3) << 17) | ((128u >> 4) << 24);
+  const int64_t grid = ceil_div(a.n, L4_OUTPUTS) * ceil_div(a.rows, ROWS);
+  if (grid > 0x7fffffff) OXB_FAIL("MatMulNBits: %lld rows", (long long)a.rows);
+  launch(umma_linear4_kernel<T, ROWS, ST>, dim3((unsigned)grid), dim3(L4_THREADS), S::kSmem, s, p);
+}
+
+template <typename T>
+void launch_prompt(const Linear4& a, cudaStream_t s) {
+  if (a.rows <= 128) a.scales_f16 ? launch_prompt<T, 128, __half>(a, s) : launch_prompt<T, 128, float>(a, s);
+  else a.scales_f16 ? launch_prompt<T, 256, __half>(a, s) : launch_prompt<T, 256, float>(a, s);
+}
+
+}  // namespace
+
+// Rows that TMA does not take as they lie (their length no multiple of 16 bytes) are copied.
+size_t linear4_workspace(const Linear4& a) { return linear4_many_rows(a) && a.k % 8 != 0 ? (size_t)a.rows * ((a.k + 7) / 8 * 8) * 2 : 0; }
+
+void linear4_prompt(const Linear4& a, cudaStream_t s) { a.dt == DT::F16 ? launch_prompt<__half>(a, s) : launch_prompt<__nv_bfloat16>(a, s); }
+
+}  // namespace k
+}  // namespace oxb

@@ -33,8 +33,8 @@ def linear_weights(gen, n, k, group, zero_points, bias):
     return w
 
 
-def linear_matrix(w, k):
-    """The [n][k] matrix in 64 bits."""
+def linear_matrix(w, k, rounded=None):
+    """The [n][k] matrix in 64 bits; `rounded` to a 16-bit type as many rows take it."""
     codes = w["weights"].astype(np.int64)
     n, blocks = codes.shape[:2]
     q = np.stack((codes & 15, codes >> 4), -1).reshape(n, blocks, -1).astype(np.float64)
@@ -42,11 +42,12 @@ def linear_matrix(w, k):
     if "zero_points" in w:
         z = w["zero_points"].astype(np.int64)
         zero = np.stack((z & 15, z >> 4), -1).reshape(n, -1)[:, :blocks].astype(np.float64)
-    return torch.from_numpy(((q - zero[:, :, None]) * w["scales"].reshape(n, blocks).astype(np.float64)[:, :, None]).reshape(n, -1)[:, :k])
+    m = torch.from_numpy(((q - zero[:, :, None]) * w["scales"].reshape(n, blocks).astype(np.float64)[:, :, None]).reshape(n, -1)[:, :k])
+    return m.to(TYPES[rounded]).double() if rounded else m
 
 
-def linear(x, w, k):
-    y = x.double() @ linear_matrix(w, k).t()
+def linear(x, w, k, rounded=None):
+    y = x.double() @ linear_matrix(w, k, rounded).t()
     return y + torch.from_numpy(w["bias"]).double() if "bias" in w else y
 
 
