@@ -4,8 +4,8 @@
 // A block has 128 outputs and up to 256 rows of x.  Outputs are the rows of the accumulator, so that a weight is an element of
 // the A operand, which tensor memory may hold: the thread of an output decodes 64 of its codes, (code - zero) * scale rounded
 // once to x's type, and writes them there, a store of 32 columns and no shared memory.  x comes through TMA as the B operand.
-// Eight warps decode (four a block of 64 inputs, in turns), one thread brings x, one issues the products.  The products of a
-// block of 64 inputs by 256 rows take 512 cycles, the decoding of its 128 x 64 codes about half of that of each scheduler.
+// Sixteen warps decode (four a block of 64 inputs, in turns), one thread brings x, one issues the products, which for a block
+// of 64 inputs by 256 rows take 512 cycles.  With eight warps a block of inputs took 800, as long as one's decoding.
 //
 // The roundings of the weights are as large as those of the result (half a step of x's type each, and independent).
 // Every wait is bounded.
@@ -22,8 +22,9 @@ namespace k {
 namespace umma {
 
 constexpr int L4_OUTPUTS = 128, L4_K = 64;
-constexpr int L4_THREADS = 320;
-constexpr int L4_WEIGHT_STAGES = 4;  // 32 columns of tensor memory each
+constexpr int L4_GROUPS = 4;  // of four warps that decode
+constexpr int L4_THREADS = L4_GROUPS * 128 + 64;
+constexpr int L4_WEIGHT_STAGES = 8;  // 32 columns of tensor memory each
 
 template <int ROWS>
 struct Linear4Shape {
@@ -31,7 +32,7 @@ struct Linear4Shape {
   static constexpr int kStages = ROWS == 256 ? 6 : 8;
   static constexpr uint32_t kSmem = kStages * kTile + 1024u;
   static constexpr uint32_t kAcc = 0, kWeights = 256;  // columns of tensor memory
-  static_assert(kStages * kTile >= 2 * 8192, "the rows leave where x was");
+  static_assert(kStages * kTile >= L4_GROUPS * 8192, "the rows leave where x was");
 };
 
 struct alignas(64) Linear4Params {
@@ -41,24 +42,65 @@ struct alignas(64) Linear4Params {
   uint32_t idesc;
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t decode_pair(uint32_t code_bits, uint32_t zero, float scale);
-// 1024 + code is exact in f16, so is code - zero; one product, one rounding (the scale is exact in f32)
+// Weights out of codes: (code - zero) * scale, rounded once.  A nibble in the low bits of a number whose last place is 1 is
+// 128 + code in bf16 and 1024 + code in f16; code - zero is exact in both.
+template <typename T, typename ST>
+struct Decoder;  // f32 scales: products in f32
 template <>
-__device__ __forceinline__ uint32_t decode_pair<__half>(uint32_t bits, uint32_t zero, float scale) {
-  const uint32_t v = bits | 0x64006400u;
-  const float2 d = __half22float2(__hsub2(*(const __half2*)&v, *(const __half2*)&zero));
-  const __half2 r = __floats2half2_rn(d.x * scale, d.y * scale);
-  return *(const uint32_t*)&r;
-}
+struct Decoder<__half, float> {
+  uint32_t zero;
+  float scale;
+  __device__ __forceinline__ Decoder(uint32_t z, float s) : zero(0x64006400u + z * 0x10001u), scale(s) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
+    const uint32_t v = bits | 0x64006400u;
+    const float2 d = __half22float2(__hsub2(*(const __half2*)&v, *(const __half2*)&zero));
+    const __half2 r = __floats2half2_rn(d.x * scale, d.y * scale);
+    return *(const uint32_t*)&r;
+  }
+};
 template <>
-__device__ __forceinline__ uint32_t decode_pair<__nv_bfloat16>(uint32_t bits, uint32_t zero, float scale) {
-  const uint32_t v = bits | 0x43004300u;
-  const __nv_bfloat162 d = __hsub2(*(const __nv_bfloat162*)&v, *(const __nv_bfloat162*)&zero);
-  const uint32_t w = *(const uint32_t*)&d;
-  const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w << 16) * scale, __uint_as_float(w & 0xffff0000u) * scale);
-  return *(const uint32_t*)&r;
-}
+struct Decoder<__nv_bfloat16, float> {
+  uint32_t zero;
+  float scale;
+  __device__ __forceinline__ Decoder(uint32_t z, float s) : zero(0x43004300u + z * 0x10001u), scale(s) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
+    const uint32_t v = bits | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*(const __nv_bfloat162*)&v, *(const __nv_bfloat162*)&zero);
+    const uint32_t w = *(const uint32_t*)&d;
+    const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w << 16) * scale, __uint_as_float(w & 0xffff0000u) * scale);
+    return *(const uint32_t*)&r;
+  }
+};
+// f16 scales: one f16 product
+template <>
+struct Decoder<__half, __half> {
+  uint32_t zero;
+  __half2 scale;
+  __device__ __forceinline__ Decoder(uint32_t z, __half s) : zero(0x64006400u + z * 0x10001u), scale(__half2half2(s)) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
+    const uint32_t v = bits | 0x64006400u;
+    const __half2 r = __hmul2(__hsub2(*(const __half2*)&v, *(const __half2*)&zero), scale);
+    return *(const uint32_t*)&r;
+  }
+};
+// An f16 scale is the sum of two bf16 numbers, of 8 bits and of what is left, at most 3.  The second's product with a number
+// below 16 has 7 bits and is exact, so that adding it to the first's is the only rounding.
+template <>
+struct Decoder<__nv_bfloat16, __half> {
+  uint32_t zero;
+  __nv_bfloat162 high, low;
+  __device__ __forceinline__ Decoder(uint32_t z, __half s) : zero(0x43004300u + z * 0x10001u) {
+    const float f = __half2float(s);
+    const __nv_bfloat16 h = __float2bfloat16_rn(f);
+    high = __bfloat162bfloat162(h);
+    low = __bfloat162bfloat162(__float2bfloat16_rn(f - __bfloat162float(h)));
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
+    const uint32_t v = bits | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(*(const __nv_bfloat162*)&v, *(const __nv_bfloat162*)&zero), r = __hfma2(d, high, __hmul2(d, low));
+    return *(const uint32_t*)&r;
+  }
+};
 
 __device__ __forceinline__ void l4_mma(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc),
@@ -73,7 +115,8 @@ __device__ __forceinline__ void l4_store32(uint32_t taddr, const uint32_t (&r)[3
       : "memory");
 }
 
-template <typename T, int ROWS, typename ST>
+// WIDE: a group is at least a block of 64 inputs, which then has one scale.
+template <typename T, int ROWS, typename ST, bool WIDE>
 __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __grid_constant__ Linear4Params p) {
   using S = Linear4Shape<ROWS>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -96,7 +139,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == 4 * L4_GROUPS) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_slot)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -112,7 +155,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
     }
   };
 
-  if (warp == 9) {
+  if (warp == 4 * L4_GROUPS + 1) {
     // ---------------- rows of x ----------------
     if (elect_one()) {
       for (int b = 0; b < p.blocks; ++b) {
@@ -126,7 +169,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
       }
     }
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == 4 * L4_GROUPS) {
     // ---------------- products ----------------
     if (elect_one()) {
       const uint64_t x_at = make_smem_desc(base, 128);
@@ -151,33 +194,44 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
     __syncwarp();
   } else {
     // ---------------- weights, then the rows' way out ----------------
-    const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int turn = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int tiles = (a.n + 63) / 64 * 4, tile = min((out0 + r) / 16, tiles - 1), in_tile = r % 8 * 2 + r % 16 / 8;
     const uint8_t* const codes = (const uint8_t*)a.codes + (int64_t)tile * p.blocks * 512 + r % 8 * 64 + r % 16 / 8 * 8;
     const ST* const scales = (const ST*)a.scales + (int64_t)tile * a.groups * 16 + in_tile;
     const uint8_t* const zeros = a.zeros ? a.zeros + (int64_t)tile * a.groups * 16 + in_tile : nullptr;
-    constexpr uint32_t kOffset = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u;
-    uint2 next[4];
+    // what a block of 64 inputs takes, fetched while the one before is decoded
+    constexpr int SCALES = WIDE ? 1 : 4;
+    struct Fetched {
+      uint2 codes[4];
+      ST scale[SCALES];  // of the block, or of its four 16 inputs; those behind the last group meet x of 0
+      uint8_t zero[SCALES];
+    } next;
     auto fetch = [&](int b) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) next[q] = *(const uint2*)(codes + (int64_t)b * 512 + q * 16);
-    };
-    if (half < p.blocks) fetch(half);
-    bool ok = true;
-    for (int b = half; b < p.blocks; b += 2) {
-      uint2 now[4];
+      for (int q = 0; q < 4; ++q) next.codes[q] = *(const uint2*)(codes + (int64_t)b * 512 + q * 16);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) now[q] = next[q];
-      if (b + 2 < p.blocks) fetch(b + 2);
-      // groups of the block's four 16 inputs; those behind the last group meet x of 0
-      float scale[4];
-      uint32_t zero[4];
+      for (int s = 0; s < SCALES; ++s) {
+        const int at = (WIDE ? b >> (p.shift - 6) : min((b * 64 + s * 16) >> p.shift, a.groups - 1)) * 16;
+        next.scale[s] = scales[at];
+        next.zero[s] = zeros ? zeros[at] : (uint8_t)8;
+      }
+    };
+    if (turn < p.blocks) fetch(turn);
+    bool ok = true;
+#pragma unroll 1
+    for (int b = turn; b < p.blocks; b += L4_GROUPS) {
+      const Fetched now = next;
+      if (b + L4_GROUPS < p.blocks) fetch(b + L4_GROUPS);
+      uint32_t w[32];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const int group = min((b * 64 + s * 16) >> p.shift, a.groups - 1);
-        scale[s] = to_f32(scales[(int64_t)group * 16]);
-        zero[s] = kOffset + (zeros ? zeros[(int64_t)group * 16] : 8u) * 0x10001u;
+        const Decoder<T, ST> decode(now.zero[WIDE ? 0 : s], now.scale[WIDE ? 0 : s]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)  // inputs 16 s + 4 q + 2 e and the next: nibbles 2 (s % 2) + e of word s / 2
+            w[8 * s + 2 * q + e] = decode((s / 2 ? now.codes[q].y : now.codes[q].x) >> (8 * (s % 2) + 4 * e) & 0x000f000fu);
       }
       const int ws = b % L4_WEIGHT_STAGES;
       if (b >= L4_WEIGHT_STAGES && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_w_empty[ws]), ((b / L4_WEIGHT_STAGES) & 1u) ^ 1u, abortp))) {
@@ -186,16 +240,6 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
         break;
       }
       tc_fence_after();
-      uint32_t w[32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t word = h ? now[q].y : now[q].x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)  // inputs 32 h + 16 (e / 2) + 4 q + 2 (e % 2) and the next
-            w[16 * h + 8 * (e / 2) + 2 * q + e % 2] = decode_pair<T>(word >> (4 * e) & 0x000f000fu, zero[2 * h + e / 2], scale[2 * h + e / 2]);
-        }
       l4_store32(tmem + lane_base + S::kWeights + ws * 32, w);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
@@ -206,24 +250,24 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
       if (lane == 0) give_up(64);
       ok = false;
     }
-    // the four warps of a half go on together or not at all
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+    // the four warps of a group go on together or not at all
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + turn) : "memory");
     if (!*abortp) {
       tc_fence_after();
       const int out = out0 + r;
       const float bias = a.bias && out < a.n ? a.bias[out] : 0.f;
-      uint8_t* const staging = base_ptr + half * 8192;  // 32 rows of 128 outputs
+      uint8_t* const staging = base_ptr + turn * 8192;  // 32 rows of 128 outputs
       const int outs = min(L4_OUTPUTS, a.n - out0);
       const bool wide = a.n % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
 #pragma unroll 1
-      for (int c = 0; c < ROWS / 64; ++c) {
-        const int first = half * (ROWS / 2) + c * 32;
+      for (int c = 0; c < ROWS / (32 * L4_GROUPS); ++c) {
+        const int first = turn * (ROWS / L4_GROUPS) + c * 32;
         uint32_t v[32];
         tmem_ld32_nowait(tmem + lane_base + S::kAcc + first, v);
         tmem_ld_wait_for(v);
 #pragma unroll
         for (int e = 0; e < 32; ++e) *(T*)(staging + e * 256 + r * 2) = from_f32<T>(__uint_as_float(v[e]) + bias);
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + turn) : "memory");
         const int i = (int)threadIdx.x & 127;
         if (wide) {
 #pragma unroll
@@ -236,7 +280,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
           for (int row = 0; row < 32; ++row)
             if (row0 + first + row < a.rows) ((T*)a.y)[(row0 + first + row) * a.n + out0 + i] = *(const T*)(staging + row * 256 + i * 2);
         }
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + turn) : "memory");
       }
     }
   }
@@ -252,7 +296,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
     }
   }
   __syncthreads();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_slot), "r"(512) : "memory");
+  if (warp == 4 * L4_GROUPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_slot), "r"(512) : "memory");
 }
 
 // Rows of odd length, or at an odd address, once more with a stride that TMA takes.
@@ -286,7 +330,7 @@ EncodeTiledFn tiled_encoder() {
   return fn;
 }
 
-template <typename T, int ROWS, typename ST>
+template <typename T, int ROWS, typename ST, bool WIDE>
 void launch_prompt(const Linear4& a, cudaStream_t s) {
   using S = Linear4Shape<ROWS>;
   static std::mutex mu;
@@ -296,7 +340,7 @@ void launch_prompt(const Linear4& a, cudaStream_t s) {
   {
     std::lock_guard<std::mutex> lock(mu);
     if (device < 0 || device >= 64 || !have[device]) {
-      OXB_CUDA(cudaFuncSetAttribute(umma_linear4_kernel<T, ROWS, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+      OXB_CUDA(cudaFuncSetAttribute(umma_linear4_kernel<T, ROWS, ST, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
       if (device >= 0 && device < 64) have[device] = true;
     }
   }
@@ -322,9 +366,11 @@ void launch_prompt(const Linear4& a, cudaStream_t s) {
   p.idesc = (1u << 4) | (type << 7) | (type << 10) | (((uint32_t)ROWS >> 3) << 17) | ((128u >> 4) << 24);
   const int64_t grid = ceil_div(a.n, L4_OUTPUTS) * ceil_div(a.rows, ROWS);
   if (grid > 0x7fffffff) OXB_FAIL("MatMulNBits: %lld rows", (long long)a.rows);
-  launch(umma_linear4_kernel<T, ROWS, ST>, dim3((unsigned)grid), dim3(L4_THREADS), S::kSmem, s, p);
+  launch(umma_linear4_kernel<T, ROWS, ST, WIDE>, dim3((unsigned)grid), dim3(L4_THREADS), S::kSmem, s, p);
 }
 
+template <typename T, int ROWS, typename ST>
+void launch_prompt(const Linear4& a, cudaStream_t s) { a.group >= L4_K ? launch_prompt<T, ROWS, ST, true>(a, s) : launch_prompt<T, ROWS, ST, false>(a, s); }
 template <typename T>
 void launch_prompt(const Linear4& a, cudaStream_t s) {
   if (a.rows <= 128) a.scales_f16 ? launch_prompt<T, 128, __half>(a, s) : launch_prompt<T, 128, float>(a, s);
