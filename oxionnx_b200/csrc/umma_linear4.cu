@@ -9,6 +9,8 @@
 //
 // The roundings of the weights are as large as those of the result (half a step of x's type each, and independent).
 // Every wait is bounded.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -21,6 +23,8 @@ namespace k {
 
 namespace umma {
 
+namespace cg = cooperative_groups;
+
 constexpr int L4_OUTPUTS = 128, L4_K = 64;
 constexpr int L4_GROUPS = 4;  // of four warps that decode
 constexpr int L4_THREADS = L4_GROUPS * 128 + 64;
@@ -32,13 +36,14 @@ struct Linear4Shape {
   static constexpr int kStages = ROWS == 256 ? 6 : 8;
   static constexpr uint32_t kSmem = kStages * kTile + 1024u;
   static constexpr uint32_t kAcc = 0, kWeights = 256;  // columns of tensor memory
-  static_assert(kStages * kTile >= L4_GROUPS * 8192, "the rows leave where x was");
+  static_assert(kStages * kTile >= ROWS * 512u, "the sums of a cluster meet where x was");
 };
 
 struct alignas(64) Linear4Params {
   CUtensorMap x;
   Linear4 a;
   int blocks, shift;  // of 64 inputs; log2 of the inputs of a group
+  int splits;         // blocks of a cluster, which share an output tile's inputs
   uint32_t idesc;
 };
 
@@ -129,8 +134,10 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
   uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
   volatile int* const abortp = &abort_flag;
   const int out_blocks = (a.n + L4_OUTPUTS - 1) / L4_OUTPUTS;
-  const int out0 = (int)(blockIdx.x % out_blocks) * L4_OUTPUTS;
-  const int64_t row0 = (int64_t)(blockIdx.x / out_blocks) * ROWS;
+  const int tile_of_grid = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
+  const int out0 = tile_of_grid % out_blocks * L4_OUTPUTS;
+  const int64_t row0 = (int64_t)(tile_of_grid / out_blocks) * ROWS;
+  const int block0 = (int)((int64_t)p.blocks * split / p.splits), blocks = (int)((int64_t)p.blocks * (split + 1) / p.splits) - block0;  // its inputs
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int i = 0; i < S::kStages; ++i) mbar_init(smem_u32(&bar_x_full[i]), 1), mbar_init(smem_u32(&bar_x_empty[i]), 1);
@@ -158,14 +165,14 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
   if (warp == 4 * L4_GROUPS + 1) {
     // ---------------- rows of x ----------------
     if (elect_one()) {
-      for (int b = 0; b < p.blocks; ++b) {
+      for (int b = 0; b < blocks; ++b) {
         const int stage = b % S::kStages;
         if (b >= S::kStages && !mbar_wait(smem_u32(&bar_x_empty[stage]), ((b / S::kStages) & 1u) ^ 1u, abortp)) {
           give_up(61);
           break;
         }
         mbar_expect_tx(smem_u32(&bar_x_full[stage]), S::kTile);
-        tma_load_2d(base + stage * S::kTile, &p.x, smem_u32(&bar_x_full[stage]), b * L4_K, (int)row0);
+        tma_load_2d(base + stage * S::kTile, &p.x, smem_u32(&bar_x_full[stage]), (block0 + b) * L4_K, (int)row0);
       }
     }
     __syncwarp();
@@ -175,7 +182,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
       const uint64_t x_at = make_smem_desc(base, 128);
       const uint32_t w_at = tmem + S::kWeights, acc = tmem + S::kAcc, idesc = p.idesc;
       bool ok = true;
-      for (int b = 0; b < p.blocks; ++b) {
+      for (int b = 0; b < blocks; ++b) {
         const int stage = b % S::kStages, ws = b % L4_WEIGHT_STAGES;
         ok = mbar_wait(smem_u32(&bar_x_full[stage]), (b / S::kStages) & 1u, abortp) && mbar_wait(smem_u32(&bar_w_full[ws]), (b / L4_WEIGHT_STAGES) & 1u, abortp);
         if (!ok) {
@@ -207,7 +214,8 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
       ST scale[SCALES];  // of the block, or of its four 16 inputs; those behind the last group meet x of 0
       uint8_t zero[SCALES];
     } next;
-    auto fetch = [&](int b) {
+    auto fetch = [&](int local) {
+      const int b = block0 + local;
 #pragma unroll
       for (int q = 0; q < 4; ++q) next.codes[q] = *(const uint2*)(codes + (int64_t)b * 512 + q * 16);
 #pragma unroll
@@ -217,12 +225,12 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
         next.zero[s] = zeros ? zeros[at] : (uint8_t)8;
       }
     };
-    if (turn < p.blocks) fetch(turn);
+    if (turn < blocks) fetch(turn);
     bool ok = true;
 #pragma unroll 1
-    for (int b = turn; b < p.blocks; b += L4_GROUPS) {
+    for (int b = turn; b < blocks; b += L4_GROUPS) {
       const Fetched now = next;
-      if (b + L4_GROUPS < p.blocks) fetch(b + L4_GROUPS);
+      if (b + L4_GROUPS < blocks) fetch(b + L4_GROUPS);
       uint32_t w[32];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
@@ -265,6 +273,11 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
         uint32_t v[32];
         tmem_ld32_nowait(tmem + lane_base + S::kAcc + first, v);
         tmem_ld_wait_for(v);
+        if (p.splits > 1) {  // f32 sums, [row][128 outputs], for the cluster
+#pragma unroll
+          for (int e = 0; e < 32; ++e) *(uint32_t*)(base_ptr + (first + e) * 512 + r * 4) = v[e];
+          continue;
+        }
 #pragma unroll
         for (int e = 0; e < 32; ++e) *(T*)(staging + e * 256 + r * 2) = from_f32<T>(__uint_as_float(v[e]) + bias);
         asm volatile("bar.sync %0, 128;" ::"r"(1 + turn) : "memory");
@@ -285,6 +298,34 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
     }
   }
 
+  // ---------------- a cluster's sums, in the order of the inputs: every block has its share of the rows ----------------
+  if (p.splits > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int outs = min(L4_OUTPUTS, a.n - out0);
+    const bool wide = a.n % 4 == 0 && ((uintptr_t)a.y & 7) == 0;
+    for (int i = threadIdx.x; i < ROWS / p.splits * 32; i += L4_THREADS) {
+      const int row = split + i / 32 * p.splits, col = i % 32 * 4;
+      if (row0 + row >= a.rows || col >= outs) continue;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < p.splits; ++c) {
+        const float4 v = *(const float4*)(cluster.map_shared_rank(base_ptr, c) + row * 512 + col * 4);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+      T out[4];
+      const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(a.bias && col + e < outs ? v[e] + a.bias[out0 + col + e] : v[e]);
+      T* const to = (T*)a.y + (row0 + row) * a.n + out0 + col;
+      if (wide) *(uint2*)to = *(const uint2*)out;
+      else
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < outs) to[e] = out[e];
+    }
+    cluster.sync();
+  }
+
   // ---------------- teardown ----------------
   tc_fence_before();
   __syncthreads();
@@ -299,13 +340,21 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
   if (warp == 4 * L4_GROUPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_slot), "r"(512) : "memory");
 }
 
-// Rows of odd length, or at an odd address, once more with a stride that TMA takes.
-__global__ void __launch_bounds__(256) linear4_pad_rows(const uint16_t* x, uint16_t* padded, int64_t rows, int k, int stride) {
+// Rows whose length is no multiple of 16 bytes, once more with a stride that is one: 16 bytes a thread.
+__global__ void __launch_bounds__(256) linear4_pad_rows(const uint16_t* x, uint16_t* padded, int rows, int k, int stride) {
   pdl_enter();
-  for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < rows * stride; i += gridDim.x * 256LL) {
-    const int64_t row = i / stride;
-    const int col = (int)(i - row * stride);
-    padded[i] = col < k ? x[row * k + col] : (uint16_t)0;
+  const int pieces = stride / 8;
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const uint16_t* const src = x + (int64_t)row * k;
+    for (int i = threadIdx.x; i < pieces; i += 256) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = i * 8 + e * 2;
+        w[e] = (at < k ? src[at] : 0u) | (at + 1 < k ? (uint32_t)src[at + 1] : 0u) << 16;
+      }
+      *(uint4*)(padded + (int64_t)row * stride + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
@@ -352,7 +401,7 @@ void launch_prompt(const Linear4& a, cudaStream_t s) {
   int64_t stride = a.k;
   if (a.workspace) {
     stride = (a.k + 7) / 8 * 8;
-    launch(linear4_pad_rows, dim3((unsigned)std::min<int64_t>(ceil_div(a.rows * stride, 256), 148 * 8)), dim3(256), 0, s, (const uint16_t*)a.x, (uint16_t*)a.workspace, a.rows, a.k, (int)stride);
+    launch(linear4_pad_rows, dim3((unsigned)std::min<int64_t>(a.rows, kDependentBlocks)), dim3(256), 0, s, (const uint16_t*)a.x, (uint16_t*)a.workspace, (int)a.rows, a.k, (int)stride);
     x = a.workspace;
   }
   const cuuint64_t dims[2] = {(cuuint64_t)a.k, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)stride * 2};
@@ -364,9 +413,27 @@ void launch_prompt(const Linear4& a, cudaStream_t s) {
   // kind::f16: f32 accumulator, A (from tensor memory) and B in x's type, both K-major, 128 x ROWS
   const uint32_t type = a.dt == DT::F16 ? 0u : 1u;
   p.idesc = (1u << 4) | (type << 7) | (type << 10) | (((uint32_t)ROWS >> 3) << 17) | ((128u >> 4) << 24);
-  const int64_t grid = ceil_div(a.n, L4_OUTPUTS) * ceil_div(a.rows, ROWS);
-  if (grid > 0x7fffffff) OXB_FAIL("MatMulNBits: %lld rows", (long long)a.rows);
-  launch(umma_linear4_kernel<T, ROWS, ST, WIDE>, dim3((unsigned)grid), dim3(L4_THREADS), S::kSmem, s, p);
+  const int64_t tiles = ceil_div(a.n, L4_OUTPUTS) * ceil_div(a.rows, ROWS);
+  if (tiles > 0x7fffffff / 8 || a.rows > 0x7fffffff) OXB_FAIL("MatMulNBits: %lld rows", (long long)a.rows);
+  // Where the tiles leave SMs idle, the inputs of each are split over a cluster, four blocks of 64 at least: 256 rows by
+  // 4096x4096 27.2 -> 14.6 us, by 8192x4096 49.4 -> 19.7, 64 rows by 4096x4096 21.7 -> 10.6, by 1024x4096 8.2 -> 8.3.  An eighth
+  // of the SMs is left out of the count, since clusters do not fill every group of SMs: 144 blocks in fours took two turns.
+  p.splits = 1;
+  while (p.splits < 8 && tiles * p.splits * 2 <= device_sms() * 7 / 8 && p.blocks >= 4 * p.splits * 2) p.splits *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.splits));
+  cfg.blockDim = dim3(L4_THREADS);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.splits > 1 ? 2 : 1;
+  OXB_CUDA(cudaLaunchKernelEx(&cfg, umma_linear4_kernel<T, ROWS, ST, WIDE>, p));
 }
 
 template <typename T, int ROWS, typename ST>

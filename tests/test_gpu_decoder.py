@@ -61,7 +61,7 @@ def check_linear(rows, k, n, group, kind, zero_points=True, bias=False, seed=0, 
     y = torch.full((rows, n), math.nan, dtype=x.dtype, device="cuda")
     s = session([linear_node(k, n, group, w)], {"x": x.cuda()}, {"y": y}, w)
     run(s)
-    many = rows > 32 and kind != "float32"  # these multiply 16-bit matrices, whose elements are rounded once
+    many = rows > 16 and kind != "float32"  # these multiply 16-bit matrices, whose elements are rounded once
     within(y, D.linear(x, w, k), D.linear_bound(x, w, k, kind, rounded_weights=many))
     if many:
         within(y, D.linear(x, w, k, rounded=kind), D.linear_bound(x, w, k, kind, rounded_weights=False) * (1 + D.half_step(kind)))
@@ -410,7 +410,7 @@ class Layer:
     def plain(self, x, new):
         """The same steps, each result rounded to the type, keys and values kept in lists."""
         dt = D.TYPES[self.kind]
-        rounded = self.kind if x.shape[0] > 32 and x.dtype != torch.float32 else None
+        rounded = self.kind if x.shape[0] > 16 and x.dtype != torch.float32 else None
         x = x.double()
         qkv = (x @ D.linear_matrix(self.w1, self.hidden, rounded).t()).to(self.dev["x"].dtype)
         q, k, v = qkv.split((self.heads * self.size, self.kv_heads * self.size, self.kv_heads * self.size), 1)
@@ -426,7 +426,7 @@ class Layer:
                     s = kk[:, head // (self.heads // self.kv_heads)] @ qq[head] / math.sqrt(self.size)
                     context[row, head] = torch.softmax(s, 0) @ vv[:, head // (self.heads // self.kv_heads)]
                 row += 1
-        rounded = self.kind if x.shape[0] > 32 else None
+        rounded = self.kind if x.shape[0] > 16 else None
         return context.flatten(1).to(dt).double() @ D.linear_matrix(self.w2, self.heads * self.size, rounded).t()
 
 
