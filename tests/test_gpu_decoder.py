@@ -649,3 +649,10 @@ def test_bindings_refuse_other_types():
         s.bind_output_device("y", y.data_ptr() + 1, y.numel(), "float16")
     with pytest.raises(OnnxError, match="holds"):
         s.bind_output_device("y", y.data_ptr(), y.numel() - 1, "float16")
+
+
+@pytest.mark.parametrize("half,interleaved,packed", [(32, False, True), (16, True, False), (0, False, False), (5, False, True)])
+def test_append_of_a_long_batch(half, interleaved, packed):
+    """Enough tokens for the kernel that serves several of them a block; idle ones among them, rows behind the last."""
+    new = [1200, 1, 700, 333, 210]
+    check_append(D.Paged(new, [1500, 0, 700, 300, 4000], 2, 1, 64, 32, "bfloat16", seed=6, behind=21, packed=packed), half, interleaved)
