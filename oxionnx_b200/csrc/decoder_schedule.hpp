@@ -19,10 +19,10 @@ namespace k {
 
 struct PromptWork {
   static constexpr int kKeys = 128;  // of a tile
-  // Steps that an item costs beside its tiles.  With 1 / 2 / 3 / 4 / 6: a prompt of 8192 tokens 622 / 521 / 489 / 493 / 501 us,
-  // seven packed ones (209 to 1746 tokens) 183 / 153 / 152 / 164 / 166 us: blocks with the short items of a prompt's
-  // beginning finish late, or early.
-  static constexpr int kBegin = 3;
+  // Steps that an item costs beside its tiles.  With 1 / 2 / 3 / 4 of them a prompt of 8192 tokens took 622 / 521 / 489 / 493 us
+  // from cold clocks, and warm 556 / 554 with 2 / 3; seven packed ones (209 to 1746 tokens) 183 / 148 / 150 / 164, one of 256
+  // tokens 27 / 35 with 2 / 3: blocks with the short items of a prompt's beginning finish late, or early.
+  static constexpr int kBegin = 2;
 
   int rows, base, span, kv_heads;  // new tokens; tokens before them (length - rows, below 0 where rows see nothing); tokens of a tile
 

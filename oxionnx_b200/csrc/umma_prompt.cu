@@ -109,6 +109,16 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// in 32 bits where both fit, as they do for all but absurd sizes: the division of 64-bit numbers is a hundred instructions
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+  return ((unsigned long long)(x | y) >> 32) ? x / y : (long long)((unsigned)x / (unsigned)y);
+}
+// The largest of three; NaN where one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -157,35 +167,39 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
     return PromptWork{(long long)s.rows * group >= p.least_rows ? s.rows : 0, s.length - s.rows, p.span, a.kv_heads};
   };
   long long total = 0, per = 0, begin = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    long long seen = 0;
-    for (int first = 0; first < a.t.sequences; first += PR_THREADS) {
-      const int b = first + (int)threadIdx.x;
-      long long mine = 0, sum;
-      if (b < a.t.sequences) {
-        bool bad;
-        mine = work_of(sequence_of(a.t, b, &bad)).total();
-      }
-      sum = mine;
+  {
+    // Up to PR_THREADS sequences a thread has its own in hand when the sum of all is known; beyond, they are gone through twice.
+    const int rounds = (a.t.sequences + PR_THREADS - 1) / PR_THREADS;
+    for (int pass = 0; pass < (rounds > 1 ? 2 : 1); ++pass) {
+      long long seen = 0;
+      for (int round = 0; round < rounds; ++round) {
+        const int b = round * PR_THREADS + (int)threadIdx.x;
+        long long mine = 0, sum;
+        if (b < a.t.sequences) {
+          bool bad;
+          mine = work_of(sequence_of(a.t, b, &bad)).total();
+        }
+        sum = mine;
 #pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const long long up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
+        for (int o = 1; o < 32; o *= 2) {
+          const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += up;
+        }
+        if (lane == 31) scan[warp] = sum;
+        __syncthreads();
+        sum += seen;
+        for (int w = 0; w < PR_THREADS / 32; ++w) {
+          if (w < warp) sum += scan[w];
+          seen += scan[w];
+        }
+        if (pass == 0 && round + 1 == rounds) {
+          total = seen;
+          per = max((long long)PR_LEAST_STEPS, quotient(total + gridDim.x - 1, gridDim.x));
+          begin = blockIdx.x * per;
+        }
+        if ((pass == 1 || rounds == 1) && begin >= sum - mine && begin < sum) start_b = b, start_before = sum - mine;
+        __syncthreads();
       }
-      if (lane == 31) scan[warp] = sum;
-      __syncthreads();
-      for (int w = 0; w < PR_THREADS / 32; ++w) {
-        if (w < warp) sum += scan[w];
-        if (w == warp) sum += seen;
-      }
-      for (int w = 0; w < PR_THREADS / 32; ++w) seen += scan[w];
-      if (pass == 1 && begin >= sum - mine && begin < sum) start_b = b, start_before = sum - mine;
-      __syncthreads();
-    }
-    if (pass == 0) {
-      total = seen;
-      per = max((long long)PR_LEAST_STEPS, (total + gridDim.x - 1) / gridDim.x);
-      begin = blockIdx.x * per;
     }
   }
   const long long stop = min(total, begin + per);
@@ -257,8 +271,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
               inside -= __shfl_sync(0xffffffffu, sum, 31);
             }
             const int steps = w.tiles(block) + PromptWork::kBegin;
-            kv = (int)(inside / steps);
-            item_at = at - inside % steps;
+            kv = (int)quotient(inside, steps);
+            item_at = at - (inside - (long long)kv * steps);
           }
           const int tiles = w.tiles(block);
           const long long item_end = item_at + tiles + PromptWork::kBegin, end = min(stop, item_end);
@@ -267,10 +281,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
             it.valid = 1, it.b = b, it.bad = bad ? 1 : 0;
             it.first = q.first, it.rows = q.rows, it.length = q.length;
             it.token0 = block * 2 * p.span, it.kv = kv;
-            it.c0 = (int)((item_at + PromptWork::kBegin) / per);
+            it.c0 = (int)quotient(item_at + PromptWork::kBegin, per);
             for (int t = 0; t < 2; ++t) {
               it.tiles[t] = w.tiles_of(block, t);
-              it.c1[t] = (int)((item_at + PromptWork::kBegin + max(it.tiles[t], 1) - 1) / per);
+              it.c1[t] = (int)quotient(item_at + PromptWork::kBegin + max(it.tiles[t], 1) - 1, per);
             }
           }
           at = end;
@@ -310,7 +324,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
       }
     } else if (warp == 9) {
       // ---------------- queries, keys and values ----------------
-      const int boxes = PR_KEYS / p.box;
+      const int boxes = PR_KEYS / p.box, box = lane % boxes, half = lane / boxes;  // a lane for each box of 64 lanes
       int n = 0;  // tiles brought so far
       uint32_t tails = 0;
       bool ok = true;
@@ -325,8 +339,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
         if (!w.valid) break;
         const int* const table = a.t.page_table + (int64_t)w.b * a.t.max_pages;
         auto page_of = [&](int j) -> int {  // of this lane's box of tile j; behind the sequence, and in place of what is no page: the zeros behind the cache
-          const int key = j * PR_KEYS + lane * p.box;
-          if (lane >= boxes || j >= w.j1 || key >= w.length) return (int)a.t.pages;
+          const int key = j * PR_KEYS + box * p.box;
+          if (half >= S::kHalves || j >= w.j1 || key >= w.length) return (int)a.t.pages;
           const int page = table[key / a.t.page];
           if (page >= 0 && page < a.t.pages) return page;
           if (!w.bad) report(a.err, kErrPage);
@@ -358,10 +372,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
             const uint32_t bar = smem_u32(&bar_full[stage]), dst = ring + stage * S::kTile;
             if (lane == 0) mbar_expect_tx(bar, S::kTile);
             __syncwarp();
-            if (lane < boxes)
-#pragma unroll
-              for (int h = 0; h < S::kHalves; ++h)
-                tma_load_4d(dst + h * 16384u + lane * p.box * 128u, kind == 0 ? &p.keys : &p.values, bar, h * 64, w.kv, (j * PR_KEYS + lane * p.box) % a.t.page, page);
+            if (lane < boxes * S::kHalves)
+              tma_load_4d(dst + half * 16384u + box * p.box * 128u, kind == 0 ? &p.keys : &p.values, bar, half * 64, w.kv, (j * PR_KEYS + box * p.box) % a.t.page, page);
           }
           page = next;
         }
@@ -392,17 +404,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
           give_up(code);
           return false;
         };
-        const uint64_t kmajor = make_smem_desc(0, 128);
+        // Whole descriptors, so that an instruction costs one addition.  One thread for both tiles of rows: their products follow
+        // one another whole, and the first is done early.  A thread for each (2048 tokens 65 -> 73 us) had them share the pipe.
+        const uint64_t queries = make_smem_desc(base, 128), keys = make_smem_desc(ring, 128);
         // values: 64 lanes by 8 keys to a swizzle atom of 1024 bytes, atoms of the next 8 keys 1024 and of the next 64 lanes 16384 behind
-        const uint64_t vmajor = ((uint64_t)(16384u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+        const uint64_t values = ((uint64_t)(16384u >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61) | (ring >> 4);
         auto full = [&](int n) { return wait(bar_full[n % S::kStages], (n / S::kStages) & 1u, 43); };
         auto scores = [&](int t, int n) {  // S_t = Q_t K^T with the keys of slot n
-          const uint32_t qa = base + t * S::kTile, ka = ring + (n % S::kStages) * S::kTile;
+          const uint64_t q_at = queries + t * (S::kTile >> 4), k_at = keys + (uint32_t)(n % S::kStages) * (S::kTile >> 4);
+          const uint32_t to = tmem + S::kScores + t * 128;
 #pragma unroll
-          for (int k = 0; k < KD / 16; ++k) {
-            const uint32_t off = (uint32_t)(k / 4) * 16384u + (uint32_t)(k % 4) * 32u;
-            tc_mma_one<KIND_F16>(tmem + S::kScores + t * 128, kmajor | (((qa + off) >> 4) & 0x3fffu), kmajor | (((ka + off) >> 4) & 0x3fffu), p.idesc_s, k > 0 ? 1u : 0u);
-          }
+          for (int k = 0; k < KD / 16; ++k)
+            tc_mma_one<KIND_F16>(to, q_at + (uint32_t)(k / 4) * 1024u + (uint32_t)(k % 4) * 2u, k_at + (uint32_t)(k / 4) * 1024u + (uint32_t)(k % 4) * 2u, p.idesc_s, k > 0 ? 1u : 0u);
           tc_commit<false>(smem_u32(&bar_scores[t]));
         };
         uint32_t probs[2] = {0, 0}, tails = 0;
@@ -434,10 +447,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
               ok = wait(bar_probs[t], probs[t]++ & 1u, 46);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t va = ring + ((n + 1) % S::kStages) * S::kTile;
+              const uint64_t v_at = values + (uint32_t)((n + 1) % S::kStages) * (S::kTile >> 4);
 #pragma unroll
               for (int k = 0; k < PR_KEYS / 16; ++k)
-                tc_mma_ts(tmem + S::kOut + t * KD, tmem + S::kScores + t * 128 + k * 8, vmajor | (((va + k * 2048u) >> 4) & 0x3fffu), p.idesc_o, j > w.j0 || k > 0 ? 1u : 0u);
+                tc_mma_ts(tmem + S::kOut + t * KD, tmem + S::kScores + t * 128 + k * 8, v_at + k * 128, p.idesc_o, k > 0 ? 1u : (j > w.j0 ? 1u : 0u));
               if (j + 1 < min(w.j1, w.tiles[t])) scores(t, n + 2);
               else tc_commit<false>(smem_u32(&bar_out[t]));
             }
@@ -457,6 +470,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_col = tmem + lane_base + S::kScores + t * 128, o_col = tmem + lane_base + S::kOut + t * KD;
     const uint64_t slope2 = both(p.slope);
+    const float growth = PR_GROWTH / p.slope;
     uint32_t done = 0, outs = 0;  // key tiles and parts of this tile of rows so far
     bool whole = true;
     for (uint32_t i = 0; whole; ++i) {
@@ -503,16 +517,17 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          mx[c] = __uint_as_float(r[c][0]);
+          mx[c] = __uint_as_float(r[c][31]);
 #pragma unroll
-          for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(r[c][e]));
+          for (int e = 0; e < 30; e += 2) mx[c] = max3(mx[c], __uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+          mx[c] = max3(mx[c], __uint_as_float(r[c][30]), mx[c]);
         }
-        const float high = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float high = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
         if (j == j0) {
           top = high;
-        } else if (__any_sync(0xffffffffu, (high - top) * p.slope > PR_GROWTH)) {
+        } else if (__any_sync(0xffffffffu, !(high <= top + growth))) {
           // these scores are complete, so is the product before them: the output may be rewritten
-          const float next = fmaxf(top, high);
+          const float next = max3(top, high, high);
           const float keep = top == -INFINITY ? 0.f : ex2((top - next) * p.slope);
           top = next;
           sum *= keep;

@@ -1,5 +1,9 @@
 """What the decoder operators' path does on the host, without a GPU: claims, the lanes of typed feeds, and models with typed
 inputs through the loader."""
+import os
+import shutil
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -51,3 +55,13 @@ def test_models_carry_typed_inputs_and_packed_weights():
     assert m.optimize(1) == 0 and m.nodes()[0].op == "MatMulNBits"
     lanes, code = m.initializers()["w"]
     assert code == _ffi.DT_U8 and np.array_equal(lanes, w.astype(np.float32))
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_the_prompt_kernels_runs_cover_every_tile_once(tmp_path):
+    exe = str(tmp_path / "prompt_schedule_check")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "host_checks", "prompt_schedule_check.cpp")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-o", exe, src], check=True)
+    out = subprocess.run([exe, "400"], capture_output=True, text=True)
+    fields = out.stdout.split()
+    assert out.returncode == 0 and int(fields[0]) > 10_000 and int(fields[2]) == 0, out.stdout
