@@ -6,7 +6,8 @@
 // 16 bytes a lane are the m16n8k16 fragments of 16 outputs by 64 inputs.  Outputs are the fragments' rows and x's rows their
 // columns, so that up to 8 rows cost no more instructions than one.  code - zero is a whole number below 16 in size and exact
 // in either 16-bit type, so the products are exact and the sums are f32; a group's sum is scaled in f32.  f32 rows are taken
-// as the sum of three bf16 numbers (8 bits of the significand each, all 24 of them), whose products are exact as well.
+// as the sum of three bf16 numbers (8 bits of the significand each, all 24 of them, cut off and not rounded, so that the largest
+// numbers stay finite), whose products are exact as well.
 //
 // A block has 16 (or 32) outputs and splits the inputs over its warps; the warps' sums meet in shared memory in one order.
 #include <cooperative_groups.h>
@@ -96,12 +97,10 @@ __device__ __forceinline__ void load4(const T* src, int left, bool whole, uint32
       float a = v[2 * i], b = v[2 * i + 1];
 #pragma unroll
       for (int s = 0; s < SPLIT; ++s) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        w[s][at + i] = *(const uint32_t*)&h;
-        // an infinity's remainder is 0, not infinity minus infinity; NaN stays in the first part
-        const float ra = a - __low2float(h), rb = b - __high2float(h);
-        a = fabsf(a) <= 3.4028235e38f && fabsf(ra) <= 3.4028235e38f ? ra : 0.f;
-        b = fabsf(b) <= 3.4028235e38f && fabsf(rb) <= 3.4028235e38f ? rb : 0.f;
+        w[s][at + i] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);  // the upper halves: 8 bits of the significand, cut off
+        // an infinity's remainder is 0, not infinity minus infinity
+        a = fabsf(a) == INFINITY ? 0.f : a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+        b = fabsf(b) == INFINITY ? 0.f : b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
       }
     }
   }
