@@ -20,6 +20,8 @@ from .graph import Graph, Node
 # TensorProto.DataType
 ONNX_DTYPE = {np.dtype(np.float32): 1, np.dtype(np.uint8): 2, np.dtype(np.int8): 3, np.dtype(np.uint16): 4, np.dtype(np.int16): 5,
               np.dtype(np.int32): 6, np.dtype(np.int64): 7, np.dtype(np.bool_): 9, np.dtype(np.float16): 10, np.dtype(np.float64): 11}
+# the types that inputs may be declared by name (bfloat16 is no numpy type)
+ONNX_NAMED = {"float32": 1, "uint8": 2, "int8": 3, "int32": 6, "float16": 10, "bfloat16": 16}
 
 
 # ---- protobuf wire format ---------------------------------------------------------------------
@@ -88,7 +90,8 @@ def _value_info(name: str, shape: Sequence, dtype) -> bytes:
             dims += _len(1, _str(2, d if isinstance(d, str) else "N"))  # dim_param
         else:
             dims += _len(1, _int(1, int(d)))  # dim_value
-    tensor_type = _int(1, ONNX_DTYPE[np.dtype(dtype)]) + _len(2, dims)
+    code = ONNX_NAMED[dtype] if isinstance(dtype, str) and dtype in ONNX_NAMED else ONNX_DTYPE[np.dtype(dtype)]
+    tensor_type = _int(1, code) + _len(2, dims)
     return _str(1, name) + _len(2, _len(1, tensor_type))
 
 
