@@ -3333,6 +3333,7 @@ void Planner::plan_paged_attention(const NodeDef& n) {
   a.err = S.err_flag_;
   if (const size_t bytes = k::paged_attention_workspace(a)) {
     a.workspace = owned_buffer(bytes);
+    S.arrival_counts_.push_back(DeviceBuffer{a.workspace, bytes});
     OXB_CUDA(cudaMemsetAsync(a.workspace, 0, bytes, C.stream()));
     OXB_CUDA(cudaStreamSynchronize(C.stream()));
   }

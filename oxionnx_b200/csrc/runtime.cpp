@@ -457,6 +457,9 @@ int Session::check_error_flag() {
     *(volatile int*)err_flag_ = 0;
     for (auto* p : umma_plans_) k::umma_plan_reset_after_error(p);
     for (auto* c : umma_chains_) k::umma_chain_reset_after_error(c);
+    // a kernel that gave up may have left its counts of parts behind
+    for (const DeviceBuffer& b : arrival_counts_) (void)cudaMemsetAsync(b.ptr, 0, b.bytes, ctx_->stream());
+    if (!arrival_counts_.empty()) (void)cudaStreamSynchronize(ctx_->stream());
   }
   return flag;
 }
@@ -489,6 +492,7 @@ void Session::begin_copies() {
 
 void Session::upload(const oxb200_operand* feeds, uint32_t n) {
   begin_copies();
+  unbind_inputs();
   for (auto& in : input_staging_) {
     const oxb200_operand* f = nullptr;
     for (uint32_t i = 0; i < n; ++i)
@@ -562,10 +566,15 @@ void Session::stage_out(void* dst, const void* src, size_t bytes) {
   OXB_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToHost, ctx_->stream()));
 }
 
-// Orders stream `s` behind the last run that was enqueued on a caller's stream.
-void Session::follow_enqueued(cudaStream_t s) {
-  if (!enqueued_ || enqueued_on_ == s) return;
+// Orders stream `s` (and a second one) behind the last run that was enqueued on a caller's stream.  Streams are told apart by
+// their ids: a new one may have a destroyed one's handle while that one's work still runs.
+void Session::follow_enqueued(cudaStream_t s, cudaStream_t also) {
+  if (!enqueued_) return;
+  unsigned long long id = 0;
+  OXB_CUDA(cudaStreamGetId(s, &id));
+  if (id == enqueued_on_) return;
   OXB_CUDA(cudaStreamWaitEvent(s, enqueued_ev_, 0));
+  if (also) OXB_CUDA(cudaStreamWaitEvent(also, enqueued_ev_, 0));
   if (s == ctx_->stream()) enqueued_ = false;
 }
 
@@ -770,6 +779,7 @@ void Session::rebind_input(int value_index, void* ptr) {
 }
 
 void Session::prepare_pipeline() {
+  unbind_inputs();
   if (pipe_ready_) return;
   // uploads and downloads have a stream each: a download waits for its run, and an upload queued behind it
   // in the same stream would wait for that run too instead of overlapping it
@@ -809,6 +819,7 @@ void Session::prepare_pipeline() {
 
 void Session::submit(const oxb200_operand* feeds, uint32_t n, bool profile) {
   prepare_pipeline();
+  follow_enqueued(ctx_->stream(), copy_stream_);
   Flight& fl = flight_[submit_idx_];
   Flight& prev = flight_[submit_idx_ ^ 1];
   if (fl.busy) raise(OXB200_FAILED, "submit: two runs are already in flight; collect one first");
@@ -1027,9 +1038,14 @@ void Session::output_device_ptr(const std::string& name, void** ptr, uint64_t* l
   raise(OXB200_FAILED, "output_device_ptr: '%s' is not an output of the planned graph", name.c_str());
 }
 
-void Session::clear_bindings() {
-  if (!own_in_ptr_.empty())
+// Inputs read the session's own buffers again, which is where host feeds go: never into a caller's.
+void Session::unbind_inputs() {
+  if (!own_in_ptr_.empty() && in_flight() == 0)
     for (size_t i = 0; i < input_staging_.size(); ++i) rebind_input(input_staging_[i].second, own_in_ptr_[i]);
+}
+
+void Session::clear_bindings() {
+  unbind_inputs();
   bound_in_.clear();
   bound_out_.clear();
 }
@@ -1090,7 +1106,7 @@ void Session::enqueue(cudaStream_t stream) {
   restore_outputs();
   if (recorded) return;
   OXB_CUDA(cudaEventRecord(enqueued_ev_, stream));
-  enqueued_on_ = stream;
+  OXB_CUDA(cudaStreamGetId(stream, &enqueued_on_));
   enqueued_ = true;
 }
 

@@ -209,9 +209,11 @@ class Session {
   void run_steps(bool profile, bool lanes_wanted, cudaStream_t stream);
   // Runs on callers' streams: the last one's end, which any other stream waits for before it touches the session's memory.
   cudaEvent_t enqueued_ev_ = nullptr;
-  cudaStream_t enqueued_on_ = nullptr;
+  unsigned long long enqueued_on_ = 0;  // id of its stream
   bool enqueued_ = false;
-  void follow_enqueued(cudaStream_t s);
+  void follow_enqueued(cudaStream_t s, cudaStream_t also = nullptr);
+  void unbind_inputs();
+  std::vector<DeviceBuffer> arrival_counts_;  // of the kernels whose parts are joined by the last to come; zero between runs
   std::vector<void*> own_in_ptr_;  // the session's own buffer of each graph input (what an unbound input reads)
   bool input_in_tensor_map(int value_index) const;
   void apply_input_bindings(cudaStream_t s);

@@ -656,3 +656,84 @@ def test_append_of_a_long_batch(half, interleaved, packed):
     """Enough tokens for the kernel that serves several of them a block; idle ones among them, rows behind the last."""
     new = [1200, 1, 700, 333, 210]
     check_append(D.Paged(new, [1500, 0, 700, 300, 4000], 2, 1, 64, 32, "bfloat16", seed=6, behind=21, packed=packed), half, interleaved)
+
+
+# ---- sizes and orders that take other ways -------------------------------------------------------
+def test_attention_of_thousands_of_streams():
+    new = [1] * 4096
+    check_attend(D.Paged(new, [1 + i % 37 for i in range(4096)], 2, 1, 64, 16, "bfloat16", seed=60))
+
+
+def test_attention_of_hundreds_of_prompts():
+    """More sequences than the prompt kernel's block has threads, of which some are streamed and some multiplied."""
+    new = [1 + (i * 7) % 40 for i in range(500)]
+    check_attend(D.Paged(new, [n + i % 90 for i, n in enumerate(new)], 4, 1, 64, 16, "float16", seed=61))
+
+
+@pytest.mark.parametrize("heads,size", [(192, 64), (130, 40), (128, 128)])
+def test_attention_with_very_many_heads_to_a_key_head(heads, size):
+    check_attend(D.Paged([3, 1], [40, 100], heads, 1, size, 16, "bfloat16", seed=62))
+
+
+def test_offsets_behind_four_gigabytes():
+    """The same small sequences at the far end of caches of 2^32 lanes and more each."""
+    p = D.Paged([1, 90], [50, 120], 8, 4, 128, 64, "bfloat16", seed=63)
+    dev = attend_inputs(p)
+    pages = 2**32 // (64 * 4 * 128) + 40
+    for name in ("key_cache", "value_cache"):
+        big = torch.empty(pages, 64, 4, 128, dtype=torch.bfloat16, device="cuda")
+        big[pages - p.pages :] = dev[name]
+        dev[name] = big
+    dev["page_table"] = torch.where(dev["page_table"] >= 0, dev["page_table"] + (pages - p.pages), dev["page_table"]).to(torch.int32)
+    out = torch.full(p.q.shape, math.nan, dtype=torch.bfloat16, device="cuda")
+    run(session([("OxiPagedAttention", "attend", list(dev), ["out"], {"num_heads": 8, "kv_num_heads": 4})], dev, {"out": out}))
+    within(out, *D.attend(p))
+    rows = {"query": p.q.cuda(), "key": p.k.cuda(), "value": p.v.cuda(), **{n: dev[n] for n in ("key_cache", "value_cache", *TABLES)}}
+    rotated = torch.empty(p.q.shape, dtype=torch.bfloat16, device="cuda")
+    run(session([("OxiPagedCacheAppend", "append", list(rows), ["r", "kc", "vc"], {"num_heads": 8, "kv_num_heads": 4})], rows, {"r": rotated}))
+    (want, _), (kc, _), vc = D.append(p, None, None, False)
+    assert torch.equal(rotated.double().cpu(), want)
+    tail = dev["value_cache"][pages - p.pages :].cpu()
+    assert torch.equal(torch.nan_to_num(tail), torch.nan_to_num(vc))
+    tail = dev["key_cache"][pages - p.pages :].double().cpu()
+    assert torch.equal(torch.nan_to_num(tail), torch.nan_to_num(kc))
+
+
+def test_linear_of_the_largest_numbers():
+    """f32 rows at the end of their range: the parts of a number round to no infinity."""
+    g = torch.Generator().manual_seed(64)
+    w = D.linear_weights(g, 33, 64, 32, False, False)
+    w["weights"][:] = 0x88  # code 8: weights of 0
+    w["weights"][:, 0, 0] = 0x89  # and one of the scale
+    x = torch.full((2, 64), torch.finfo(torch.float32).max)
+    x[1] = 0.0
+    x[1, 0] = -torch.finfo(torch.float32).max
+    y = torch.empty(2, 33, device="cuda")
+    run(session([linear_node(64, 33, 32, w)], {"x": x.cuda()}, {"y": y}, w))
+    within(y, D.linear(x, w, 64), 4 * 2.0**-23 * D.linear(x, w, 64).abs())
+
+
+def test_host_feeds_never_go_into_bound_buffers():
+    p = D.Paged([1, 90], [50, 90], 4, 2, 64, 16, "float16", seed=65)
+    p.kc, p.vc = torch.nan_to_num(p.kc), torch.nan_to_num(p.vc)
+    s, dev, out = check_attend(p)
+    want, kept = out.clone(), {n: t.clone() for n, t in dev.items()}
+    feeds = {n: (t.float() if t.is_floating_point() else t).cpu().numpy() for n, t in dev.items()}
+    feeds["query"] = feeds["query"] * 0.5
+    other = s.run(feeds)["out"]
+    assert not np.array_equal(other, want.float().cpu().numpy())
+    assert np.array_equal(s.run_pipelined([feeds, feeds])[1]["out"], other)
+    assert all(torch.equal(kept[n], dev[n]) for n in dev)
+    out.zero_()
+    run(s)  # the bindings still hold
+    assert torch.equal(out, want)
+
+
+def test_models_with_typed_inputs_through_the_loader():
+    p = D.Paged([1, 20], [50, 20], 4, 2, 64, 16, "bfloat16", seed=66)
+    p.kc, p.vc = torch.nan_to_num(p.kc), torch.nan_to_num(p.vc)
+    s, dev, out = check_attend(p)
+    feeds = {n: (t.float() if t.is_floating_point() else t).cpu().numpy() for n, t in dev.items()}
+    b = Session.builder().with_input_types({n: name_of(t) for n, t in dev.items()}).with_input_shapes({n: tuple(t.shape) for n, t in dev.items()})
+    loaded = b.with_optimization_level(1).build_from_graph(s.graph, {})
+    assert np.array_equal(loaded.run(feeds)["out"], out.float().cpu().numpy())
