@@ -154,6 +154,38 @@ typedef struct {
 
 /* ---- pure predicates (no device) ---------------------------------------------------- */
 
+/* Operators of decoders.  Tensors are row-major; "16-bit" means f16 or bf16.  What is not stated here is declined.
+ *
+ * MatMulNBits: y[m][n] = sum over groups g of scale[n][g] * sum over k in g of x[m][k] (code[n][k] - zero[n][g]) + bias[n]
+ *   inputs   x [.., K] f32 or 16-bit; codes u8 [N][groups][block_size / 2], the even input's code in the low nibble; scales
+ *            [N][groups]; optional zero points u8 [N][ceil(groups / 2)], packed like the codes (8 without); an omitted group
+ *            index; optional bias [N].  All but x are initializers.
+ *   attrs    K, N, bits = 4, block_size (a power of two, 16 .. 1024)
+ *   output   [.., N] in x's type.  Sums are f32.  17 rows and more of 16 bits multiply weights that are rounded once to x's
+ *            type; fewer, and f32 rows, exact ones.
+ *
+ * The paged operators share five inputs.  A cache is [pages][page][kv_heads][size], 16-bit, pages of a multiple of 16 tokens,
+ * heads of a multiple of 8 lanes up to 256.  cu_query i32 [sequences + 1]: the new rows' bounds, from 0 up.  Rows behind the
+ * last bound, and new rows beyond a sequence's length (idle streams have length 0), are not appended; their results are 0.
+ * kv_lengths i32 [sequences]: a sequence's tokens with its new ones.  page_table i32
+ * [sequences][n]: the page of its tokens p * page ..; entries behind its length are not read.  These are device values: bounds
+ * out of order, lengths beyond the table and pages outside the cache leave memory alone, give the rows concerned zeros at
+ * best, and are reported by the next call that waits.
+ *
+ * OxiPagedCacheAppend: inputs query [.., heads * size], key and value [.., kv_heads * size] (or, with these two omitted, one
+ *   product [.., (heads + 2 kv_heads) * size]), key cache, value cache, cu_query, kv_lengths, page_table, optional cos and sin
+ *   f32 [positions][half].  The first 2 * half lanes of queries and keys are rotated by the token's position (pairs half apart,
+ *   or side by side with interleaved = 1), in f32; rows are f32 or the caches' type.
+ *   attrs num_heads, kv_num_heads, interleaved.  Outputs: the rotated queries in the caches' type, and the two
+ *   caches, which are graph inputs updated where they lie: what reads them afterwards reads these outputs.
+ *   Two sequences that append to one slot leave either's row there.
+ * OxiPagedAttention: inputs query [.., heads * size] (f32 is rounded to the caches' type), key cache, value cache, cu_query,
+ *   kv_lengths, page_table.  Row i of a sequence's n new ones sees its tokens 0 .. kv_lengths - n + i; a row that sees none
+ *   gets zeros.  attrs num_heads, kv_num_heads, scale (1 / sqrt(size)), max_query_length (a promise on the new tokens of a
+ *   sequence, checked on the device; 0: none).  Output [.., heads * size] in the caches' type.  Results do not depend on the
+ *   order in which blocks finish.  A NaN or an infinity among a sequence's later values may reach earlier rows of the same call,
+ *   whose probabilities for them are 0; what lies in a page behind the sequence does not. */
+
 /* oxionnx_cuda::is_supported_op (src/lib.rs:217).  Adds the INT8 family the reference's
  * own CUDA provider never claimed. */
 int oxb200_is_supported_op(const char* op_type);

@@ -9,7 +9,9 @@
 // as the sum of three bf16 numbers (8 bits of the significand each, all 24 of them, cut off and not rounded, so that the largest
 // numbers stay finite), whose products are exact as well.
 //
-// A block has 16 (or 32) outputs and splits the inputs over its warps; the warps' sums meet in shared memory in one order.
+// A block has 16 (or 64) outputs and splits the inputs over its warps; the warps' sums meet in shared memory in one order.
+// 1 x 4096 x 16384 takes 12.5 us, where the codes alone stream in 7.3: the decoding (about 106 instructions for 16 outputs by 64
+// inputs) is not hidden entirely.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -20,6 +20,10 @@
 // when the last scores of this one are done, and its first scores run while this one's output leaves.  An item that a border
 // between blocks cuts leaves its parts in the workspace, and whoever brings the last part joins them in the order of the keys.
 // Every wait is bounded.
+//
+// A step (both tiles by 128 keys of 128 lanes) takes 4000 cycles, of which the products are 2048 and the exponentials as many:
+// 8192 tokens of 32 heads on 8 take 553 us, 995 TFLOP/s, at the power cap.  64 keys a step in two buffers (products of 64
+// columns run at half rate), polynomials for a part of the exponentials and a second issuing thread were no faster.
 #include <algorithm>
 #include <mutex>
 
