@@ -41,6 +41,21 @@ __device__ __forceinline__ Sequence sequence_of(const PagedTables& t, int b, boo
   return Sequence{first, end - first, length};
 }
 
+// The lowest nibbles of both halves of `w`, and `offset` beside them: a nibble in the low bits of a number whose last place is 1
+// is 128 + code in bf16 and 1024 + code in f16.  One instruction; out of (w & mask) | constant the compiler made two, and the
+// stream of 4096 x 65536 codes took 41.7 us in place of 36.8.
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t offset) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(offset));
+  return r;
+}
+// A constant in a register, of which the compiler does not know that it is one.
+__device__ __forceinline__ uint32_t in_register(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 __device__ __forceinline__ void report(int* err, int code) { *(volatile int*)err = code; }
 
 }  // namespace k

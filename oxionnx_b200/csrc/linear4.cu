@@ -9,12 +9,15 @@
 // as the sum of three bf16 numbers (8 bits of the significand each, all 24 of them, cut off and not rounded, so that the largest
 // numbers stay finite), whose products are exact as well.
 //
-// A block has 16 (or 64) outputs and splits the inputs over its warps; the warps' sums meet in shared memory in one order.
-// 1 x 4096 x 16384 takes 12.5 us, where the codes alone stream in 7.3: the decoding (about 106 instructions for 16 outputs by 64
-// inputs) is not hidden entirely.
+// A block has 16, 32 or 64 outputs and splits the inputs over its warps; the warps' sums meet in shared memory in one order.
+// Rows that fit shared memory over many inputs have a kernel of their own, whose blocks stay (linear4_stream): 1 x 4096 x 16384
+// takes 10.0 us in place of 11.5, 1 x 4096 x 65536 30, 4.6 TB/s.  What bounds both is the decoding, about 80 instructions for 16
+// outputs by 64 inputs, of which 28 run on the pipe of shifts and logic at half rate.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "decoder_device.cuh"
 
@@ -51,7 +54,7 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A nibble in the low bits of a number whose last place is 1: 128 + code in bf16, 1024 + code in f16.
+// Where `nibbles` puts them: into 128 in bf16, 1024 in f16.
 template <typename H>
 constexpr uint32_t kOffset = 0;
 template <>
@@ -121,6 +124,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear4_rows(Linear4 a, int64_t r
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int tile0 = blockIdx.x / splits * MT, slice = blockIdx.x % splits * kWarps + warp, blocks = (a.k + 63) / 64;
   row0 += (int64_t)blockIdx.y * NT * 8;
+  const uint32_t offset = in_register(kOffset<H>);
   const int first = (int)((int64_t)blocks * slice / (splits * kWarps)), last = (int)((int64_t)blocks * (slice + 1) / (splits * kWarps));
   const int rows = (int)min((int64_t)NT * 8, a.rows - row0);
   const bool aligned = a.k % 4 == 0 && ((uintptr_t)a.x & 15) == 0;
@@ -188,10 +192,10 @@ __global__ void __launch_bounds__(kWarps * 32) linear4_rows(Linear4 a, int64_t r
           // words: steps 0 and 1, 2 and 3 of row g, the same of row g + 8
           const uint32_t w0 = (j < 2 ? w[m].x : w[m].y) >> (j & 1) * 8, w1 = (j < 2 ? w[m].z : w[m].w) >> (j & 1) * 8;
           uint32_t f[4];
-          f[0] = minus<H>((w0 & 0x000f000fu) | kOffset<H>, z0);
-          f[1] = minus<H>((w1 & 0x000f000fu) | kOffset<H>, z1);
-          f[2] = minus<H>((w0 >> 4 & 0x000f000fu) | kOffset<H>, z0);
-          f[3] = minus<H>((w1 >> 4 & 0x000f000fu) | kOffset<H>, z1);
+          f[0] = minus<H>(nibbles(w0, offset), z0);
+          f[1] = minus<H>(nibbles(w1, offset), z1);
+          f[2] = minus<H>(nibbles(w0 >> 4, offset), z0);
+          f[3] = minus<H>(nibbles(w1 >> 4, offset), z1);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -248,6 +252,249 @@ __global__ void __launch_bounds__(kWarps * 32) linear4_rows(Linear4 a, int64_t r
   }
 }
 
+// ---- few rows of many inputs ----
+// One block an SM takes an equal run of output tiles, two at a time, and its warps the inputs, the same ones of every tile: x is
+// laid out once in shared memory as the lanes take it, and each warp streams its part of the codes, scales and zero points
+// through a ring of its own (cp.async, a stage for up to four 64-input blocks of two tiles), so that the decoding of some hides
+// behind the stream of others.
+constexpr int kStreamWarps = 16;
+
+template <int SUB, bool ZP, typename ST>
+struct Stream {
+  // a stage: [tile of two][block][512 bytes of codes], then [tile][block][group of the block][16 scales], then zero points alike
+  static constexpr int kChunk = SUB == 4 ? 2 : 4;
+  static constexpr int kScaleBytes = 16 * (int)sizeof(ST), kUnits = 2 * kChunk;
+  static constexpr int kScales = kUnits * 512, kZeros = kScales + kUnits * SUB * kScaleBytes;
+  static constexpr int kStage = kZeros + (ZP ? kUnits * SUB * 16 : 0);
+  static constexpr int kStages = kStage * kStreamWarps * 3 <= 176 << 10 ? 3 : 2;
+  static constexpr int kRing = kStage * kStages;
+  static constexpr int kSums = 16 * kStreamWarps * 16 * 4;  // bytes of one of two halves: the sums of 16 tiles of a row, or of two of 8 rows
+  static constexpr int kMostX = (227 << 10) - 2 * kSums - kRing * kStreamWarps;
+};
+
+__device__ __forceinline__ void stream16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <typename T, int SUB, bool ZP, typename ST>
+__global__ void __launch_bounds__(kStreamWarps * 32, 1) linear4_stream(Linear4 a, int shift, int x_bytes) {
+  using S = Stream<SUB, ZP, ST>;
+  constexpr int STEPS = 4 / SUB, kChunk = S::kChunk;
+  const uint32_t offset = in_register(kOffset<T>);
+  extern __shared__ __align__(128) uint8_t smem[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int blocks = (a.k + 63) / 64, tiles = (a.n + 15) / 16, rows = (int)a.rows;
+  const int t0 = (int)((int64_t)tiles * blockIdx.x / gridDim.x), t1 = (int)((int64_t)tiles * (blockIdx.x + 1) / gridDim.x);
+  const int first = (int)((int64_t)blocks * warp / kStreamWarps), last = (int)((int64_t)blocks * (warp + 1) / kStreamWarps);
+  const uint32_t ring_offset = x_bytes + 2 * S::kSums + warp * S::kRing, ring_at = (uint32_t)__cvta_generic_to_shared(smem) + ring_offset;
+
+  // the next stage to bring: tile, first block, place
+  int f_tile = first < last ? t0 : t1, f_block = first;
+  uint32_t f_stage = 0;
+  const int tile_codes = blocks * 512;  // K below 2^24
+  auto fetch = [&]() {
+    if (f_tile < t1) {
+      const int n = min(kChunk, last - f_block), pair = min(2, t1 - f_tile);
+      const uint32_t dst = ring_at + f_stage;
+      const uint8_t* const src = (const uint8_t*)a.codes + ((int64_t)f_tile * tile_codes + (f_block * 512 + lane * 16));
+      if (n == kChunk && pair == 2) {
+#pragma unroll
+        for (int c = 0; c < kChunk; ++c) stream16(dst + lane * 16 + c * 512, src + c * 512), stream16(dst + lane * 16 + (kChunk + c) * 512, src + tile_codes + c * 512);
+      } else {
+        for (int m = 0; m < pair; ++m)
+          for (int c = 0; c < n; ++c) stream16(dst + lane * 16 + (m * kChunk + c) * 512, src + (m * tile_codes + c * 512));
+      }
+      // 16 bytes a lane: groups of a block, each in sizeof(ST) pieces of scales and one of zero points
+      auto group_of = [&](int c, int s) { return SUB == 1 ? (f_block + c) >> shift : min((f_block + c) * SUB + s, a.groups - 1); };  // behind the last x is 0
+#pragma unroll
+      for (int i0 = 0; i0 < S::kUnits * SUB * (int)sizeof(ST); i0 += 32) {
+        const int i = i0 + lane, piece = i % (int)sizeof(ST), s = i / (int)sizeof(ST) % SUB, c = i / ((int)sizeof(ST) * SUB) % kChunk, m = i / ((int)sizeof(ST) * SUB * kChunk);
+        if (m < pair && c < n) stream16(dst + S::kScales + i * 16, (const uint8_t*)a.scales + (((int64_t)(f_tile + m) * a.groups + group_of(c, s)) * S::kScaleBytes + piece * 16));
+      }
+      if constexpr (ZP) {
+#pragma unroll
+        for (int i0 = 0; i0 < S::kUnits * SUB; i0 += 32) {
+          const int i = i0 + lane, s = i % SUB, c = i / SUB % kChunk, m = i / (SUB * kChunk);
+          if (m < pair && c < n) stream16(dst + S::kZeros + i * 16, a.zeros + ((int64_t)(f_tile + m) * a.groups + group_of(c, s)) * 16);
+        }
+      }
+      f_stage = f_stage + S::kStage == (uint32_t)S::kRing ? 0 : f_stage + S::kStage;
+      f_block += n;
+      if (f_block == last) f_block = first, f_tile += 2;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // the weights are the session's own: they need not wait for the kernel in front
+#pragma unroll
+  for (int i = 0; i < S::kStages; ++i) fetch();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // x as [steps 0 and 1, 2 and 3][row][block][lane of a quarter][8], zeros behind K; an odd number of blocks keeps rows on other banks
+  const int row_bytes = (blocks | 1) * 64, half_bytes = rows * row_bytes;
+  const bool whole = a.k % 8 == 0 && ((uintptr_t)a.x & 15) == 0;
+  constexpr int kAtOnce = 4;  // rows whose loads are in flight together
+#pragma unroll 1
+  for (int i = threadIdx.x; i < blocks * 8; i += kStreamWarps * 32) {  // 8 lanes of x: two lanes of a quarter
+    uint8_t* const dst = smem + (i >> 2 & 1) * half_bytes + (i >> 3) * 64 + (i & 1) * 32 + (i >> 1 & 1) * 8;
+#pragma unroll 1
+    for (int row0 = 0; row0 < rows; row0 += kAtOnce) {
+      const T* const src = (const T*)a.x + ((int64_t)row0 * a.k + i * 8);
+      uint4 v[kAtOnce];
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r) {
+        v[r] = make_uint4(0, 0, 0, 0);
+        if (row0 + r >= rows) continue;
+        if (whole) {
+          if (i * 8 < a.k) v[r] = *(const uint4*)(src + (int64_t)r * a.k);
+        } else {
+          uint32_t w[1][8];
+          load4<T, 1>(src + (int64_t)r * a.k, a.k - i * 8, false, w, 0);
+          load4<T, 1>(src + (int64_t)r * a.k + 4, a.k - i * 8 - 4, false, w, 2);
+          v[r] = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r)
+        if (row0 + r < rows) {
+          *(uint2*)(dst + (row0 + r) * row_bytes) = make_uint2(v[r].x, v[r].y);
+          *(uint2*)(dst + (row0 + r) * row_bytes + 16) = make_uint2(v[r].z, v[r].w);
+        }
+    }
+  }
+  __syncthreads();
+  const uint32_t x_at = min(g, rows - 1) * row_bytes + q * 16;  // rows behind the last are copies of it: their columns of the products go nowhere
+
+  uint32_t stage = 0;
+  int slot = 0, half = 0;
+  const int slots = 16 / rows & ~1;  // tiles whose sums meet at a time: two at least
+  for (int tile = t0; tile < t1; tile += 2) {
+    const bool two = tile + 1 < t1;
+    float acc[2][4] = {};
+    for (int b0 = first; b0 < last; b0 += kChunk) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+      __syncwarp();
+      const uint8_t *const at = smem + ring_offset + stage, *const codes = at + lane * 16, *const scales = at + S::kScales + 2 * g * (int)sizeof(ST), *const zeros = at + S::kZeros + 2 * g;
+      stage = stage + S::kStage == (uint32_t)S::kRing ? 0 : stage + S::kStage;
+      auto x_of = [&](int c, uint32_t (&x)[8]) {
+        const uint8_t* const src = smem + (x_at + b0 * 64) + c * 64;
+        *(uint4*)&x[0] = *(const uint4*)src;
+        *(uint4*)&x[4] = *(const uint4*)(src + half_bytes);
+      };
+      auto unit = [&](int m, int c, const uint32_t (&x)[8], float (&sum)[4]) {
+        const int u = m * kChunk + c;
+        const uint4 w = *(const uint4*)(codes + u * 512);
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          float scale0, scale1;
+          if constexpr (sizeof(ST) == 2) {
+            const float2 v = __half22float2(*(const __half2*)(scales + (u * SUB + s) * S::kScaleBytes));
+            scale0 = v.x, scale1 = v.y;
+          } else {
+            const float2 v = *(const float2*)(scales + (u * SUB + s) * S::kScaleBytes);
+            scale0 = v.x, scale1 = v.y;
+          }
+          uint32_t z0 = kOffset<T> + 0x00080008u, z1 = z0;
+          if constexpr (ZP) {
+            const uint32_t both = *(const uint16_t*)(zeros + (u * SUB + s) * 16);
+            z0 = kOffset<T> + (both & 15u) * 0x10001u, z1 = kOffset<T> + (both >> 8) * 0x10001u;
+          }
+          float part[4] = {};
+#pragma unroll
+          for (int j = s * STEPS; j < (s + 1) * STEPS; ++j) {
+            const uint32_t w0 = (j < 2 ? w.x : w.y) >> (j & 1) * 8, w1 = (j < 2 ? w.z : w.w) >> (j & 1) * 8;
+            uint32_t f[4];
+            f[0] = minus<T>(nibbles(w0, offset), z0);
+            f[1] = minus<T>(nibbles(w1, offset), z1);
+            f[2] = minus<T>(nibbles(w0 >> 4, offset), z0);
+            f[3] = minus<T>(nibbles(w1 >> 4, offset), z1);
+            mma<T>(part, f, x[2 * j], x[2 * j + 1]);
+          }
+          sum[0] += part[0] * scale0, sum[1] += part[1] * scale0;
+          sum[2] += part[2] * scale1, sum[3] += part[3] * scale1;
+        }
+      };
+      auto units = [&](auto count) {  // without a branch between them, so that they overlap
+#pragma unroll
+        for (int c = 0; c < decltype(count)::value; ++c) {
+          uint32_t x[8];
+          x_of(c, x);
+          unit(0, c, x, acc[0]);
+          unit(1, c, x, acc[1]);
+        }
+      };
+      const int n = min(kChunk, last - b0);
+      if (two && n == kChunk) {
+        units(std::integral_constant<int, kChunk>());
+      } else if (two && n == 3 && kChunk > 3) {
+        units(std::integral_constant<int, 3>());
+      } else if (two && n == 2) {
+        units(std::integral_constant<int, 2>());
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < n; ++c) {
+          uint32_t x[8];
+          x_of(c, x);
+          unit(0, c, x, acc[0]);
+          if (two) unit(1, c, x, acc[1]);
+        }
+      }
+      __syncwarp();  // all lanes have read the stage
+      fetch();
+    }
+    float* const meet = (float*)(smem + x_bytes + half * S::kSums);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = q * 2 + (e & 1);
+        if (row < rows) meet[(((slot + m) * kStreamWarps + warp) * rows + row) * 16 + g + (e >> 1) * 8] = acc[m][e];
+      }
+    slot += 2;
+    if (slot < slots && tile + 2 < t1) continue;
+    __syncthreads();  // the other half's sums have been taken: who takes them passes here afterwards
+    for (int i = threadIdx.x; i < slot * rows * 16; i += kStreamWarps * 32) {
+      const int o = i % 16, row = i / 16 % rows, which = i / 16 / rows, n = (tile + 2 - slot + which) * 16 + o;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kStreamWarps; ++w) sum += meet[((which * kStreamWarps + w) * rows + row) * 16 + o];
+      if (n < min(a.n, t1 * 16)) ((T*)a.y)[(int64_t)row * a.n + n] = from_f32<T>(a.bias ? sum + a.bias[n] : sum);
+    }
+    slot = 0, half ^= 1;
+  }
+}
+
+template <typename T, int SUB, bool ZP, typename ST>
+bool launch_stream(const Linear4& a, cudaStream_t s) {
+  using S = Stream<SUB, ZP, ST>;
+  const int64_t x_bytes = a.rows * (ceil_div(a.k, 64) | 1) * 128;
+  if (x_bytes > S::kMostX) return false;
+  static std::mutex mu;
+  static bool have[64] = {};
+  int device = 0, shift = 0;
+  OXB_CUDA(cudaGetDevice(&device));
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (device < 0 || device >= 64 || !have[device]) {
+      OXB_CUDA(cudaFuncSetAttribute(linear4_stream<T, SUB, ZP, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kMostX + 2 * S::kSums + S::kRing * kStreamWarps));
+      if (device >= 0 && device < 64) have[device] = true;
+    }
+  }
+  while ((64 << shift) < a.group) ++shift;
+  launch(linear4_stream<T, SUB, ZP, ST>, dim3((unsigned)std::min<int64_t>(device_sms(), ceil_div(a.n, 16))), dim3(kStreamWarps * 32),
+         (size_t)x_bytes + 2 * S::kSums + S::kRing * kStreamWarps, s, a, shift, (int)x_bytes);
+  return true;
+}
+template <typename T, int SUB>
+bool launch_stream(const Linear4& a, cudaStream_t s) {
+  if (a.scales_f16) return a.zeros ? launch_stream<T, SUB, true, __half>(a, s) : launch_stream<T, SUB, false, __half>(a, s);
+  return a.zeros ? launch_stream<T, SUB, true, float>(a, s) : launch_stream<T, SUB, false, float>(a, s);
+}
+template <typename T>
+bool launch_stream(const Linear4& a, cudaStream_t s) {  // false: x does not fit
+  return a.group == 16 ? launch_stream<T, 4>(a, s) : a.group == 32 ? launch_stream<T, 2>(a, s) : launch_stream<T, 1>(a, s);
+}
+
 template <typename T, int MT, int NT, int SUB, bool ZP, typename ST>
 void launch_rows(const Linear4& a, int64_t row0, int64_t rows, cudaStream_t s) {
   // The inputs are split over as many blocks as bring the grid to two blocks an SM, while a warp keeps two 64-input blocks.
@@ -282,16 +529,22 @@ void launch_rows(const Linear4& a, int64_t row0, int64_t rows, cudaStream_t s) {
 }
 template <typename T>
 void launch_rows(const Linear4& a, cudaStream_t s) {
-  // Tiles of 16 outputs for a warp, in us at rows x K x N, 1 / 2 / 4 tiles: 1 x 4096 x 16384 17.9 / 13.4 / 12.5, 8 x 4096 x 4096
-  // 10.9 / 8.9 / 6.4, 16 x 4096 x 4096 10.8 / 10.1 / 8.5, where rows are fetched once for all of them; small matrices want the
-  // blocks: 1 x 1024 x 1024 2.3 / 2.5 / 3.0, 5 x 1000 x 1111 (f32) 3.6 / 3.9 / 4.5; and so do 32 rows, whose fragments fill the
-  // registers: 32 x 4096 x 4096 12.9 / 16.2 / 18.2.
+  // Tiles of 16 outputs for a warp, in us at rows x K x N, 1 / 2 / 4 tiles: 1 x 1024 x 16384 5.8 / 5.3 / 3.8, 4 x 4096 x 16384
+  // (f32) 32 / 25 / 18, 8 x 2048 x 8192 7.6 / 5.4 / 5.5, where rows are fetched once for all of them; with two fragments of rows
+  // 16 x 4096 x 4096 10.3 / 7.2 / 8.2, 32 x 4096 x 4096 (f32) 32 / 22 / 25, but 16 x 4096 x 16384 - / 17.2 / 14.0, whose outputs alone
+  // give every SM a block of 4; small matrices want the blocks: 1 x 1024 x 1024
+  // 2.3 / 2.5 / 3.0, 5 x 1000 x 1111 (f32) 3.6 / 3.9 / 4.5.
   const bool large = (int64_t)a.n * a.k >= 148LL * 65536;
+  // The stream against the blocks below, in us: 1 x 4096 x 16384 10.0 / 11.5, 4 rows 10.8 / 11.8, 1 x 4096 x 4096 4.0 / 4.9,
+  // 1 x 4096 x 65536 30 / 44, 1 x 2048 x 2048 2.8 / 4.2, 8 rows 3.4 / 5.2, 1 x 2880 x 5120 5.1 / 5.8; with few inputs a warp's turn
+  // is too short: 1 x 2048 x 16384 7.8 / 6.4, 1 x 1024 x 1024 2.2 / 2.3, 1 x 512 x 2048 2.5 / 2.0.
+  if constexpr (sizeof(T) == 2)
+    if (a.rows <= 8 && a.k >= (large ? 2560 : 2048) && launch_stream<T>(a, s)) return;
   // grid.y holds 65535 blocks of rows
   for (int64_t row0 = 0; row0 < a.rows; row0 += 65535LL * 16) {
     const int64_t rows = std::min<int64_t>(a.rows - row0, 65535LL * 16);
     if (rows <= 8) large ? launch_rows<T, 4, 1>(a, row0, rows, s) : launch_rows<T, 1, 1>(a, row0, rows, s);
-    else if (rows <= 16 || sizeof(T) == 4) large ? launch_rows<T, 4, 2>(a, row0, rows, s) : launch_rows<T, 1, 2>(a, row0, rows, s);
+    else if (rows <= 16 || sizeof(T) == 4) large ? a.n >= 64 * 148 ? launch_rows<T, 4, 2>(a, row0, rows, s) : launch_rows<T, 2, 2>(a, row0, rows, s) : launch_rows<T, 1, 2>(a, row0, rows, s);
     else launch_rows<T, 1, 4>(a, row0, rows, s);
   }
 }
@@ -299,7 +552,7 @@ void launch_rows(const Linear4& a, cudaStream_t s) {
 }  // namespace
 
 // 16-bit rows from here on run on tcgen05 (umma_linear4.cu), whose block takes 128 outputs by up to 256 rows.  This file's kernel
-// against that one, at 4096x4096: 16 rows 8.5 / 9.8 us, 32 rows 13.0 / 10.2, 64 rows 24.9 / 10.4.
+// against that one, at 4096x4096: 16 rows 7.2 / 9.8 us, 32 rows 13.0 / 10.2, 64 rows 24.9 / 10.4.
 constexpr int64_t kManyRows = 17;
 
 bool linear4_many_rows(const Linear4& a) { return a.dt != DT::F32 && a.rows >= kManyRows; }

@@ -48,8 +48,7 @@ struct alignas(64) Linear4Params {
   uint32_t idesc;
 };
 
-// Weights out of codes: (code - zero) * scale, rounded once.  A nibble in the low bits of a number whose last place is 1 is
-// 128 + code in bf16 and 1024 + code in f16; code - zero is exact in both.
+// Weights out of codes: (code - zero) * scale, rounded once.  code - zero is exact in both types.
 template <typename T, typename ST>
 struct Decoder;  // f32 scales: products in f32
 template <>
@@ -57,8 +56,8 @@ struct Decoder<__half, float> {
   uint32_t zero;
   float scale;
   __device__ __forceinline__ Decoder(uint32_t z, float s) : zero(0x64006400u + z * 0x10001u), scale(s) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
-    const uint32_t v = bits | 0x64006400u;
+  __device__ __forceinline__ uint32_t operator()(uint32_t w, uint32_t offset) const {
+    const uint32_t v = nibbles(w, offset);
     const float2 d = __half22float2(__hsub2(*(const __half2*)&v, *(const __half2*)&zero));
     const __half2 r = __floats2half2_rn(d.x * scale, d.y * scale);
     return *(const uint32_t*)&r;
@@ -69,11 +68,11 @@ struct Decoder<__nv_bfloat16, float> {
   uint32_t zero;
   float scale;
   __device__ __forceinline__ Decoder(uint32_t z, float s) : zero(0x43004300u + z * 0x10001u), scale(s) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
-    const uint32_t v = bits | 0x43004300u;
+  __device__ __forceinline__ uint32_t operator()(uint32_t w, uint32_t offset) const {
+    const uint32_t v = nibbles(w, offset);
     const __nv_bfloat162 d = __hsub2(*(const __nv_bfloat162*)&v, *(const __nv_bfloat162*)&zero);
-    const uint32_t w = *(const uint32_t*)&d;
-    const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(w << 16) * scale, __uint_as_float(w & 0xffff0000u) * scale);
+    const uint32_t x = *(const uint32_t*)&d;
+    const __nv_bfloat162 r = __floats2bfloat162_rn(__uint_as_float(x << 16) * scale, __uint_as_float(x & 0xffff0000u) * scale);
     return *(const uint32_t*)&r;
   }
 };
@@ -83,8 +82,8 @@ struct Decoder<__half, __half> {
   uint32_t zero;
   __half2 scale;
   __device__ __forceinline__ Decoder(uint32_t z, __half s) : zero(0x64006400u + z * 0x10001u), scale(__half2half2(s)) {}
-  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
-    const uint32_t v = bits | 0x64006400u;
+  __device__ __forceinline__ uint32_t operator()(uint32_t w, uint32_t offset) const {
+    const uint32_t v = nibbles(w, offset);
     const __half2 r = __hmul2(__hsub2(*(const __half2*)&v, *(const __half2*)&zero), scale);
     return *(const uint32_t*)&r;
   }
@@ -101,8 +100,8 @@ struct Decoder<__nv_bfloat16, __half> {
     high = __bfloat162bfloat162(h);
     low = __bfloat162bfloat162(__float2bfloat16_rn(f - __bfloat162float(h)));
   }
-  __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
-    const uint32_t v = bits | 0x43004300u;
+  __device__ __forceinline__ uint32_t operator()(uint32_t w, uint32_t offset) const {
+    const uint32_t v = nibbles(w, offset);
     const __nv_bfloat162 d = __hsub2(*(const __nv_bfloat162*)&v, *(const __nv_bfloat162*)&zero), r = __hfma2(d, high, __hmul2(d, low));
     return *(const uint32_t*)&r;
   }
@@ -227,6 +226,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
       }
     };
     if (turn < blocks) fetch(turn);
+    const uint32_t offset = in_register(std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u);
     bool ok = true;
 #pragma unroll 1
     for (int b = turn; b < blocks; b += L4_GROUPS) {
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int e = 0; e < 2; ++e)  // inputs 16 s + 4 q + 2 e and the next: nibbles 2 (s % 2) + e of word s / 2
-            w[8 * s + 2 * q + e] = decode((s / 2 ? now.codes[q].y : now.codes[q].x) >> (8 * (s % 2) + 4 * e) & 0x000f000fu);
+            w[8 * s + 2 * q + e] = decode((s / 2 ? now.codes[q].y : now.codes[q].x) >> (8 * (s % 2) + 4 * e), offset);
       }
       const int ws = b % L4_WEIGHT_STAGES;
       if (b >= L4_WEIGHT_STAGES && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_w_empty[ws]), ((b / L4_WEIGHT_STAGES) & 1u) ^ 1u, abortp))) {

@@ -737,3 +737,26 @@ def test_models_with_typed_inputs_through_the_loader():
     b = Session.builder().with_input_types({n: name_of(t) for n, t in dev.items()}).with_input_shapes({n: tuple(t.shape) for n, t in dev.items()})
     loaded = b.with_optimization_level(1).build_from_graph(s.graph, {})
     assert np.array_equal(loaded.run(feeds)["out"], out.float().cpu().numpy())
+
+
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("rows,k,n,group,zero_points,bias", [(1, 4096, 2600, 128, True, True), (3, 1030, 9500, 16, True, False), (8, 2080, 4801, 32, False, True), (9, 1500, 6600, 64, True, True),
+                                                             (16, 4100, 2400, 32, True, False), (13, 1024, 9500, 16, False, True), (2, 70001, 150, 256, True, False), (1, 8192, 1200, 1024, False, False), (16, 10000, 1000, 128, True, True)])
+def test_linear_of_large_matrices(rows, k, n, group, zero_points, bias, kind):
+    """Whole and cut blocks and groups, rows that fill shared memory and more than that, tiles that do not come out even."""
+    s, x, y, w = check_linear(rows, k, n, group, kind, zero_points=zero_points, bias=bias, seed=rows + n)
+    first = y.clone()
+    for _ in range(3):
+        run(s)
+    assert torch.equal(first, y)
+
+
+def test_linear_of_a_large_matrix_with_scales_beyond_f16():
+    g = torch.Generator().manual_seed(71)
+    for group in (16, 32, 128):
+        w = D.linear_weights(g, 2401, 4111, group, True, True)
+        w["scales"] = (w["scales"].astype(np.float32) * np.float32(1.00001)).astype(np.float32)
+        x = torch.randn(5, 4111, generator=g).bfloat16()
+        y = torch.empty(5, 2401, dtype=torch.bfloat16, device="cuda")
+        run(session([linear_node(4111, 2401, group, w)], {"x": x.cuda()}, {"y": y}, w))
+        within(y, D.linear(x, w, 4111), D.linear_bound(x, w, 4111, "bfloat16", rounded_weights=False))
