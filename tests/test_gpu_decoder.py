@@ -760,3 +760,50 @@ def test_linear_of_a_large_matrix_with_scales_beyond_f16():
         y = torch.empty(5, 2401, dtype=torch.bfloat16, device="cuda")
         run(session([linear_node(4111, 2401, group, w)], {"x": x.cuda()}, {"y": y}, w))
         within(y, D.linear(x, w, 4111), D.linear_bound(x, w, 4111, "bfloat16", rounded_weights=False))
+
+
+def test_host_runs_follow_enqueued_ones():
+    """run and the pipelined form right behind runs on another stream: the session's buffers are not theirs before."""
+    p = D.Paged([1500, 1], [1500, 3000], 8, 2, 128, 16, "bfloat16", seed=72)
+    p.kc, p.vc = torch.nan_to_num(p.kc), torch.nan_to_num(p.vc)
+    s, dev, out = check_attend(p)
+    want = out.clone()
+    feeds = {n: (t.float() if t.is_floating_point() else t).cpu().numpy() for n, t in dev.items()}
+    other = {**feeds, "query": feeds["query"] * 0.5}
+    half = s.run(other)["out"]
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        out.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(8):
+            s.enqueue(side.cuda_stream)
+        assert np.array_equal(s.run(other)["out"], half)
+        side.synchronize()
+        assert torch.equal(out, want)
+        out.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(8):
+            s.enqueue(side.cuda_stream)
+        assert all(np.array_equal(r["out"], half) for r in s.run_pipelined([other, other, other]))
+        side.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_linears_of_two_sessions_at_once():
+    """The streaming kernel has no state of its own: two sessions on two streams, one of them replayed from a graph."""
+    a, xa, ya, _ = check_linear(2, 4096, 2600, 32, "bfloat16", seed=73)
+    b, xb, yb, _ = check_linear(7, 2500, 6000, 128, "float16", seed=74)
+    wa, wb = ya.clone(), yb.clone()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=one):
+        a.enqueue(torch.cuda.current_stream().cuda_stream)
+    ya.zero_(), yb.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(one):
+            graph.replay()
+        b.enqueue(two.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(ya, wa) and torch.equal(yb, wb)
