@@ -11,7 +11,8 @@ namespace k {
 
 // First statement of a kernel launched with `launch`: the successor may set itself up from here on (a tensor-core
 // kernel has about a microsecond of barriers, tensor memory, weight loads and instruction misses to get out of the
-// way), and nothing is read or written before the predecessor's results are visible.
+// way), and nothing is read or written before the predecessor's results are visible.  A kernel that allocates tensor memory
+// calls it behind the allocation: the successor's blocks may take columns before their wait, and keep them until this grid ends.
 __device__ __forceinline__ void pdl_enter() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -164,7 +164,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  pdl_enter();
+  // The successor is let in only behind the allocation below: a block of it that fits beside this one and takes its columns of
+  // tensor memory first would hold them until this grid ends, which this block's allocation would then never let it.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- all sequences' steps, and the sequence that this block's first step lies in ----
   auto work_of = [&](const Sequence& s) {
@@ -216,6 +218,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = tmem_base_slot;
   auto give_up = [&](int code) {
     if (!*abortp) {

@@ -1,0 +1,35 @@
+"""Rules that the device code keeps and that no run may be made to break, read from the sources."""
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "oxionnx_b200", "csrc")
+
+
+def functions(name):
+    """(name, body without comments) of every kernel and inlined device procedure of a source file."""
+    with open(os.path.join(CSRC, name)) as fh:
+        text = re.sub(r"//[^\n]*", "", fh.read())
+    text = re.sub(r"__launch_bounds__\([^{;]*?\)\s+(?=\w+\()", "", text)
+    for m in re.finditer(r"(?:__global__|__device__ __forceinline__)\s+void\s+(\w+)\([^{;]*\{", text):
+        depth, at = 1, m.end()
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[at], 0)
+            at += 1
+        yield m.group(1), text[m.end() : at]
+
+
+SOURCES = sorted(f for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")))
+
+
+def test_kernels_let_their_successor_in_behind_their_tensor_memory():
+    """A dependent grid starts once every block of this one has said so, and may take tensor memory before it waits.  Said in
+    front of the block's own allocation, that allocation can wait for columns which the successor holds until this grid ends."""
+    seen = 0
+    for source in SOURCES:
+        for name, body in functions(source):
+            alloc = [m.start() for m in re.finditer(r"tcgen05\.alloc", body)]
+            lets_in = [m.start() for m in re.finditer(r"griddepcontrol\.launch_dependents|pdl_enter\(\)", body)]
+            if alloc and lets_in:
+                seen += 1
+                assert min(lets_in) > max(alloc), f"{source}: {name}"
+    assert seen >= 5
