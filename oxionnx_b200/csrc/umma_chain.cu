@@ -351,9 +351,8 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) umma_chain_kernel(const __gr
         }
       }
       // Peers may still be reading this CTA's partial sums.  Between layers the grid barrier below covers that (a
-      // peer arrives there only after its reads, and nothing overwrites the partial sums before it); the last
-      // layer has no grid barrier, and the CTA's shared memory must outlive the peers' reads.
-      if (l + 1 == p.n_layers) cluster_sync_all();
+      // peer arrives there only after its reads, and nothing overwrites the partial sums before it); behind the
+      // last one the teardown's cluster barrier does.
     }
     if (l + 1 < p.n_layers) {
       // every CTA's rows of this layer are visible (also to the TMA unit) before anybody loads the next layer's
@@ -370,6 +369,8 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) umma_chain_kernel(const __gr
   }
 
   // ---------------- teardown ----------------
+  // A CTA's shared memory outlives its peers' reads, whichever layers its cluster had work in and whether or not it gave up.
+  if (clustered) cluster_sync_all();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

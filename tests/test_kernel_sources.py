@@ -33,3 +33,16 @@ def test_kernels_let_their_successor_in_behind_their_tensor_memory():
                 seen += 1
                 assert min(lets_in) > max(alloc), f"{source}: {name}"
     assert seen >= 5
+
+
+def test_blocks_that_others_read_from_leave_together():
+    """Shared memory that the peers of a cluster read goes away with its block: the last thing that all of the cluster does,
+    outside of any branch that depends on a block's own work or on its having given up, is a barrier of the cluster."""
+    for source, name in (("umma_chain.cu", "umma_chain_kernel"), ("linear4.cu", "linear4_rows"), ("umma_linear4.cu", "umma_linear4_kernel")):
+        body = dict(functions(source))[name]
+        reads = [m.start() for m in re.finditer(r"ld_dsmem_v4\(|map_shared_rank\(", body)]
+        barriers = [m.start() for m in re.finditer(r"cluster_sync_all\(\)|cluster\.sync\(\)", body)]
+        assert reads and barriers and barriers[-1] > reads[-1], source
+        depth = body[: barriers[-1]].count("{") - body[: barriers[-1]].count("}")
+        assert depth <= 1, f"{source}: the last barrier of the cluster stands inside of {depth} blocks"
+    assert "if (clustered) cluster_sync_all();" in dict(functions("umma_chain.cu"))["umma_chain_kernel"]
