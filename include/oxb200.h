@@ -177,7 +177,8 @@ typedef struct {
  *   f32 [positions][half].  The first 2 * half lanes of queries and keys are rotated by the token's position (pairs half apart,
  *   or side by side with interleaved = 1), in f32; rows are f32 or the caches' type.
  *   attrs num_heads, kv_num_heads, interleaved.  Outputs: the rotated queries in the caches' type, and the two
- *   caches, which are graph inputs updated where they lie: what reads them afterwards reads these outputs.
+ *   caches, which are graph inputs updated where they lie: what reads them afterwards reads these outputs.  Views of an input
+ *   (Reshape, Identity) may stand in front; nothing else may read the input or a view of it, and the two are two inputs.
  *   Two sequences that append to one slot leave either's row there.
  * OxiPagedAttention: inputs query [.., heads * size] (f32 is rounded to the caches' type), key cache, value cache, cu_query,
  *   kv_lengths, page_table.  Row i of a sequence's n new ones sees its tokens 0 .. kv_lengths - n + i; a row that sees none

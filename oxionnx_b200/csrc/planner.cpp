@@ -314,6 +314,16 @@ class Planner {
       C.counters.kernel_launches++;
     };
   }
+  // What the graph calls a value.
+  const std::string& graph_name(int vi) const {
+    for (const auto& typed : typed_index_)
+      if (typed.second == vi) return typed.first;
+    return S.values_[vi].name;
+  }
+  int root_of(int vi) const {
+    while (S.values_[vi].alias_of >= 0) vi = S.values_[vi].alias_of;
+    return vi;
+  }
   int typed_value_of(const std::string& name) {
     auto it = typed_index_.find(name);
     return it == typed_index_.end() ? value_of(name) : it->second;
@@ -3224,14 +3234,17 @@ void Planner::plan_paged_append(const NodeDef& n) {
   const char* name = n.name.c_str();
   PagedInputs p = paged_inputs(n, 3);
   if (n.outputs.size() != 3 || n.outputs[0].empty() || n.outputs[1].empty() || n.outputs[2].empty()) OXB_DECLINE("OxiPagedCacheAppend '%s': three outputs", name);
-  if (p.kc == p.vc) OXB_DECLINE("OxiPagedCacheAppend '%s': one buffer for keys and values", name);
-  for (size_t i = 3; i < 5; ++i) {
-    auto it = consumers_.find(in_name(n, i));
-    int root = i == 3 ? p.kc : p.vc;
-    while (V(root).alias_of >= 0) root = V(root).alias_of;
-    if (!V(root).is_graph_input || V(root).host) OXB_DECLINE("OxiPagedCacheAppend '%s': a cache must be a graph input", name);
-    if (it->second.size() != 1 || graph_outputs_.count(in_name(n, i)))
-      OXB_DECLINE("OxiPagedCacheAppend '%s': '%s' is updated where it lies; what else reads it must read the output", name, in_name(n, i).c_str());
+  if (root_of(p.kc) == root_of(p.vc)) OXB_DECLINE("OxiPagedCacheAppend '%s': one buffer for keys and values", name);
+  for (int vi : {p.kc, p.vc}) {
+    const Value& root = V(root_of(vi));
+    if (!root.is_graph_input || root.host) OXB_DECLINE("OxiPagedCacheAppend '%s': a cache must be a graph input", name);
+    // from the input through its views (Reshape, Identity, an append's output) to this node, each has one reader: the next
+    for (int at = vi; at >= 0; at = V(at).alias_of) {
+      const std::string& held = graph_name(at);
+      auto it = consumers_.find(held);
+      if (it == consumers_.end() || it->second.size() != 1 || graph_outputs_.count(held))
+        OXB_DECLINE("OxiPagedCacheAppend '%s': '%s' is updated where it lies; what else reads it must read the output", name, held.c_str());
+    }
   }
   const bool packed = !has_in(n, 1) && !has_in(n, 2);
   if (has_in(n, 1) != has_in(n, 2)) OXB_DECLINE("OxiPagedCacheAppend '%s': key without value", name);

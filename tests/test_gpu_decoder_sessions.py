@@ -6,6 +6,8 @@ import pytest
 
 import decoder_oracle as D
 import test_gpu_decoder as G
+from oxionnx_b200.graph import Graph, Node
+from oxionnx_b200.session import Declined, Session
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -31,3 +33,57 @@ def test_prompts_in_front_of_a_small_product(sequences):
         z.fill_(math.nan)
         G.run(s)
         G.within(z, want @ w.double(), bound)
+
+
+# ---- views of a cache ----------------------------------------------------------------------------
+SHAPES = {"query": (3, 256), "key": (3, 128), "value": (3, 128), "key_cache": (5, 16, 2, 64), "value_cache": (5, 16, 2, 64), "cu_query": (3,), "kv_lengths": (2,), "page_table": (2, 3)}
+HEADS = {"num_heads": 4, "kv_num_heads": 2}
+
+
+def append_node(kc, vc, out="", name="append"):
+    return Node("OxiPagedCacheAppend", name, ["query", "key", "value", kc, vc, *G.TABLES], ["a" + out, "b" + out, "c" + out], HEADS)
+
+
+def view(src, dst, op="Identity"):
+    return Node(op, f"{src}-{dst}", [src, "cache_shape"] if op == "Reshape" else [src], [dst], {})
+
+
+@pytest.mark.parametrize("nodes,outs,match", [
+    # another reader of the input behind the view, a graph output out of it, the input itself as an output
+    ([view("key_cache", "k"), append_node("k", "value_cache"), Node("OxiPagedAttention", "t", ["a", "key_cache", "c", *G.TABLES], ["y"], HEADS)], ["y"], "updated where it lies"),
+    ([view("key_cache", "k"), append_node("k", "value_cache"), view("key_cache", "y")], ["a", "y"], "updated where it lies"),
+    ([view("key_cache", "k", "Reshape"), append_node("k", "value_cache"), view("key_cache", "y")], ["a", "y"], "updated where it lies"),
+    ([view("value_cache", "v"), append_node("key_cache", "v")], ["a", "value_cache"], "updated where it lies"),
+    ([view("key_cache", "k"), view("k", "l"), append_node("l", "value_cache")], ["a", "k"], "updated where it lies"),
+    # two appends on two views, one of them of the cache from before the other
+    ([view("key_cache", "k"), append_node("k", "value_cache"), view("key_cache", "l"), append_node("l", "c", "2", "again")], ["a", "a2"], "updated where it lies"),
+    # one input as both caches
+    ([view("key_cache", "k"), view("key_cache", "l"), append_node("k", "l")], ["a"], "one buffer for keys and values"),
+    ([view("key_cache", "k"), append_node("k", "key_cache")], ["a"], "one buffer for keys and values"),
+])
+def test_append_refuses_views_of_a_cache_that_something_else_reads(nodes, outs, match):
+    used = {i for n in nodes for i in n.inputs} | set(outs)
+    inputs = [n for n in SHAPES if n in used]
+    types = {n: "int32" if n in G.TABLES else "float16" for n in inputs}
+    weights = {"cache_shape": torch.tensor(SHAPES["key_cache"]).float().numpy()}
+    with pytest.raises(Declined, match=match):
+        Session.builder().with_input_shapes({n: SHAPES[n] for n in inputs}).with_input_types(types).build_from_graph(Graph(nodes, inputs, outs), weights).ensure_planned()
+
+
+def test_append_through_views_that_nothing_else_reads():
+    """A chain of views in front and two appends in a row, the second on the first one's outputs."""
+    p = D.Paged([2, 1], [20, 3], 4, 2, 64, 16, "float16", seed=81)
+    dev = {"query": p.q.cuda(), "key": p.k.cuda(), "value": p.v.cuda(), "flat": p.kc.reshape(-1).cuda(), "value_cache": p.vc.cuda(), "cu_query": p.cu.cuda(), "kv_lengths": p.len.cuda(),
+           "page_table": p.table.cuda()}
+    out = torch.full(p.q.shape, math.nan, dtype=torch.float16, device="cuda")
+    heads = {"num_heads": 4, "kv_num_heads": 2}
+    nodes = [("Reshape", "r", ["flat", "cache_shape"], ["k"], {}), ("Identity", "i", ["k"], ["l"], {}),
+             ("OxiPagedCacheAppend", "one", ["query", "key", "value", "l", "value_cache", *G.TABLES], ["a", "b", "c"], heads),
+             ("OxiPagedCacheAppend", "two", ["query", "key", "value", "b", "c", *G.TABLES], ["a2", "b2", "c2"], heads)]
+    s = G.session(nodes, dev, {"a2": out}, {"cache_shape": torch.tensor(p.kc.shape).float().numpy()})
+    G.run(s)
+    (rotated, bound), (kc, _), vc = D.append(p, None, None, False)
+    G.within(out, rotated, bound)
+    got = dev["flat"].view(kc.shape).double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(kc)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(kc))
+    assert torch.equal(torch.nan_to_num(dev["value_cache"].cpu()), torch.nan_to_num(vc))
