@@ -453,15 +453,17 @@ void Session::sync() {
 // the host reads it like any other word (a copy of it out of device memory was a second fence per run, 10 us).
 int Session::check_error_flag() {
   const int flag = *(volatile int*)err_flag_;
-  if (flag != 0) {
-    *(volatile int*)err_flag_ = 0;
-    for (auto* p : umma_plans_) k::umma_plan_reset_after_error(p);
-    for (auto* c : umma_chains_) k::umma_chain_reset_after_error(c);
-    // a kernel that gave up may have left its counts of parts behind
-    for (const DeviceBuffer& b : arrival_counts_) (void)cudaMemsetAsync(b.ptr, 0, b.bytes, ctx_->stream());
-    if (!arrival_counts_.empty()) (void)cudaStreamSynchronize(ctx_->stream());
-  }
+  if (flag != 0) reset_after_error();
   return flag;
+}
+
+// Behind a run that reported something, with none of the session's kernels in flight: what they may have left half done.
+void Session::reset_after_error() {
+  *(volatile int*)err_flag_ = 0;
+  for (auto* p : umma_plans_) k::umma_plan_reset_after_error(p);
+  for (auto* c : umma_chains_) k::umma_chain_reset_after_error(c);
+  for (const DeviceBuffer& b : arrival_counts_) (void)cudaMemsetAsync(b.ptr, 0, b.bytes, ctx_->stream());  // counts of parts
+  if (!arrival_counts_.empty()) (void)cudaStreamSynchronize(ctx_->stream());
 }
 
 // The host lanes of a feed for graph input `v`, checked against the plan: f32 lanes for an input declared f32, typed
@@ -890,9 +892,7 @@ void Session::collect(oxb200_result* fetches, uint32_t n) {
     OXB_CUDA(cudaStreamSynchronize(ctx_->stream()));
     OXB_CUDA(cudaStreamSynchronize(down_stream_));
     if (other.busy) other.poisoned = true;
-    *(volatile int*)err_flag_ = 0;
-    for (auto* p : umma_plans_) k::umma_plan_reset_after_error(p);
-    for (auto* c : umma_chains_) k::umma_chain_reset_after_error(c);
+    reset_after_error();
     raise(OXB200_FAILED, "a kernel reported code %d during a pipelined run (or the run before it failed while this one was in flight); results are not valid", flag);
   }
   for (uint32_t i = 0; i < n; ++i) {

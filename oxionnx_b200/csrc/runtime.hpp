@@ -213,6 +213,7 @@ class Session {
   bool enqueued_ = false;
   void follow_enqueued(cudaStream_t s, cudaStream_t also = nullptr);
   void unbind_inputs();
+  void reset_after_error();
   std::vector<DeviceBuffer> arrival_counts_;  // of the kernels whose parts are joined by the last to come; zero between runs
   std::vector<void*> own_in_ptr_;  // the session's own buffer of each graph input (what an unbound input reads)
   bool input_in_tensor_map(int value_index) const;

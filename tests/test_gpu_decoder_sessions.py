@@ -1,16 +1,46 @@
 """The decoder operators inside sessions: what stands next to them, what order their runs keep, what is left when one fails, and
 which graphs are refused."""
+import ctypes
 import math
+import os
+import shutil
+import subprocess
 
+import numpy as np
 import pytest
 
 import decoder_oracle as D
 import test_gpu_decoder as G
 from oxionnx_b200.graph import Graph, Node
-from oxionnx_b200.session import Declined, Session
+from oxionnx_b200.session import Declined, OnnxError, Session
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="session")
+def session_state(tmp_path_factory):
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    lib = str(tmp_path_factory.mktemp("session_state") / "session_state.so")
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "host_checks", "session_state.cpp")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fPIC", "-shared", "-I/usr/local/cuda/include", "-o", lib, src], check=True)
+    w = ctypes.CDLL(lib)
+    w.error_word.restype = ctypes.POINTER(ctypes.c_int)
+    w.error_word.argtypes = w.add_failing_step.argtypes = w.drop_last_step.argtypes = [ctypes.c_void_p]
+    w.arrival_counts.restype = ctypes.c_uint32
+    w.arrival_counts.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_uint64), ctypes.c_uint32]
+    return w
+
+
+def device_words(ptr, count):
+    """`count` int32 of device memory as a tensor over them."""
+    holder = type("", (), {"__cuda_array_interface__": {"shape": (count,), "typestr": "<i4", "data": (ptr, False), "version": 3, "strides": None}})()
+    return torch.as_tensor(holder, device="cuda")
+
+
+def host_feeds(dev):
+    return {n: (t.float() if t.is_floating_point() else t).cpu().numpy() for n, t in dev.items()}
 
 
 # ---- beside kernels that hold tensor memory ------------------------------------------------------
@@ -87,3 +117,32 @@ def test_append_through_views_that_nothing_else_reads():
     got = dev["flat"].view(kc.shape).double().cpu()
     assert torch.equal(torch.isnan(got), torch.isnan(kc)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(kc))
     assert torch.equal(torch.nan_to_num(dev["value_cache"].cpu()), torch.nan_to_num(vc))
+
+
+# ---- after a kernel has given up -----------------------------------------------------------------
+@pytest.mark.parametrize("way", ["collect", "run", "wait", "resident"])
+def test_a_run_that_gave_up_leaves_no_counts_of_parts(session_state, way):
+    """The error word set as a bounded wait that ran out sets it, counts of parts left as a block that gave up leaves them:
+    whichever call reports it clears them, so that the next run does not join parts too early."""
+    p = D.Paged([1, 300], [3000, 1500], 8, 2, 128, 16, "bfloat16", seed=82)
+    p.kc, p.vc = torch.nan_to_num(p.kc), torch.nan_to_num(p.vc)
+    s, dev, out = G.check_attend(p)
+    want = out.float().cpu().numpy()
+    feeds = host_feeds(dev)
+    ptr, size = (ctypes.c_void_p * 4)(), (ctypes.c_uint64 * 4)()
+    assert session_state.arrival_counts(s.ctx.handle, ptr, size, 4) == 1
+    words = device_words(ptr[0], size[0] // 4)
+    s.run(feeds)
+    if way == "collect":
+        s.submit(feeds)
+    elif way == "wait":
+        s.enqueue(0)
+    torch.cuda.synchronize()
+    words.fill_(1)
+    torch.cuda.synchronize()
+    session_state.error_word(s.ctx.handle)[0] = 43
+    with pytest.raises(OnnxError, match="43"):
+        {"collect": s.collect, "run": s.download, "wait": s.wait, "resident": lambda: s.run_resident(0)}[way]()
+    torch.cuda.synchronize()
+    assert int(words.count_nonzero()) == 0, "counts of parts are left behind"
+    assert np.array_equal(s.run(feeds)["out"], want)
