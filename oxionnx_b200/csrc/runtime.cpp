@@ -404,6 +404,7 @@ Session::~Session() {
   cudaStreamSynchronize(ctx_->stream());
   if (enqueued_) cudaEventSynchronize(enqueued_ev_);
   if (enqueued_ev_) cudaEventDestroy(enqueued_ev_);
+  if (own_ev_) cudaEventDestroy(own_ev_);
   for (auto* p : umma_plans_) k::umma_plan_destroy(p);
   for (auto* g : umma_groups_) k::umma_group_destroy(g);
   for (auto* c : umma_chains_) k::umma_chain_destroy(c);
@@ -443,6 +444,7 @@ void Session::sync() {
   std::vector<PendingCopy> out;
   out.swap(pending_out_);
   OXB_CUDA(e);
+  own_open_ = false;
   for (const PendingCopy& c : out) std::memcpy(c.dst, c.src, c.bytes);
   out.clear();
   pending_out_.swap(out);  // keeps the allocation
@@ -485,7 +487,7 @@ static const void* feed_lanes(const oxb200_operand& f, const Value& v, const cha
 
 // A run that failed half way leaves copies in the staging memory that nobody will collect.
 void Session::begin_copies() {
-  follow_enqueued(ctx_->stream());
+  begin_own_work();
   if (small_stage_used_ == 0 && pending_out_.empty()) return;
   pending_out_.clear();
   OXB_CUDA(cudaStreamSynchronize(ctx_->stream()));
@@ -568,16 +570,37 @@ void Session::stage_out(void* dst, const void* src, size_t bytes) {
   OXB_CUDA(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToHost, ctx_->stream()));
 }
 
-// Orders stream `s` (and a second one) behind the last run that was enqueued on a caller's stream.  Streams are told apart by
-// their ids: a new one may have a destroyed one's handle while that one's work still runs.
-void Session::follow_enqueued(cudaStream_t s, cudaStream_t also) {
+// The context's stream is about to work on the session's memory: behind the last run that was enqueued on a caller's stream, and
+// (until the host has waited for it, sync) in front of the next one, whatever becomes of the call.  A second stream goes along.
+void Session::begin_own_work(cudaStream_t also) {
+  own_open_ = true;
   if (!enqueued_) return;
-  unsigned long long id = 0;
-  OXB_CUDA(cudaStreamGetId(s, &id));
-  if (id == enqueued_on_) return;
-  OXB_CUDA(cudaStreamWaitEvent(s, enqueued_ev_, 0));
+  OXB_CUDA(cudaStreamWaitEvent(ctx_->stream(), enqueued_ev_, 0));
   if (also) OXB_CUDA(cudaStreamWaitEvent(also, enqueued_ev_, 0));
-  if (s == ctx_->stream()) enqueued_ = false;
+  enqueued_ = false;  // the context's stream stands for it
+}
+
+// Orders a caller's stream behind the last run on another one and behind the context's stream.  Streams are told apart by their
+// ids: a new one may have a destroyed one's handle while that one's work still runs.
+void Session::follow_earlier_runs(cudaStream_t s) {
+  if (enqueued_) {
+    unsigned long long id = 0;
+    OXB_CUDA(cudaStreamGetId(s, &id));
+    if (id != enqueued_on_) OXB_CUDA(cudaStreamWaitEvent(s, enqueued_ev_, 0));
+  }
+  if (own_open_) {
+    if (!own_ev_) OXB_CUDA(cudaEventCreateWithFlags(&own_ev_, cudaEventDisableTiming));
+    OXB_CUDA(cudaEventRecord(own_ev_, ctx_->stream()));
+    OXB_CUDA(cudaStreamWaitEvent(s, own_ev_, 0));
+    own_open_ = false;  // the run's own event stands for it
+  }
+}
+
+// What is in `s` so far is a run of this session, complete or not.
+void Session::end_enqueued(cudaStream_t s) {
+  OXB_CUDA(cudaEventRecord(enqueued_ev_, s));
+  OXB_CUDA(cudaStreamGetId(s, &enqueued_on_));
+  enqueued_ = true;
 }
 
 static bool skipped(const Step& st, bool lanes_wanted, const std::vector<char>& typed) {
@@ -664,7 +687,7 @@ void Session::run_steps(bool profile, bool lanes_wanted, cudaStream_t s) {
   const bool on_own_stream = s == nullptr;
   if (on_own_stream) {
     s = ctx_->stream();
-    follow_enqueued(s);
+    begin_own_work();
   }
   // recordings are made and replayed on the context's stream; a caller that wants one of its own stream captures it itself
   if (graph_allowed_ && !profile && ctx_->cfg().cuda_graph && !ctx_->cfg().verify && on_own_stream && replay_graph(lanes_wanted, s)) return;
@@ -743,7 +766,7 @@ void Session::fetch_value(const std::string& name, oxb200_result* out) {
   write_result_shape(*v, out);
   if (!out->lanes) return;
   require_not_typed(name);
-  follow_enqueued(ctx_->stream());
+  begin_own_work();
   if (out->cap < (uint64_t)v->numel()) raise(OXB200_FAILED, "fetch_value: buffer too small for '%s'", name.c_str());
   int64_t n = v->numel();
   if (n == 0) return;
@@ -821,7 +844,7 @@ void Session::prepare_pipeline() {
 
 void Session::submit(const oxb200_operand* feeds, uint32_t n, bool profile) {
   prepare_pipeline();
-  follow_enqueued(ctx_->stream(), copy_stream_);
+  begin_own_work(copy_stream_);
   Flight& fl = flight_[submit_idx_];
   Flight& prev = flight_[submit_idx_ ^ 1];
   if (fl.busy) raise(OXB200_FAILED, "submit: two runs are already in flight; collect one first");
@@ -1093,21 +1116,19 @@ void Session::enqueue(cudaStream_t stream) {
   OXB_CUDA(cudaStreamIsCapturing(stream, &capturing));
   const bool recorded = capturing != cudaStreamCaptureStatusNone;
   if (!enqueued_ev_ && !recorded) OXB_CUDA(cudaEventCreateWithFlags(&enqueued_ev_, cudaEventDisableTiming));
-  if (!recorded) follow_enqueued(stream);
-  apply_input_bindings(stream);
-  point_outputs();
+  if (!recorded) follow_earlier_runs(stream);
   try {
+    apply_input_bindings(stream);
+    point_outputs();
     run_steps(false, false, stream);
     copy_outputs(stream);
   } catch (...) {
     restore_outputs();
+    if (!recorded) end_enqueued(stream);
     throw;
   }
   restore_outputs();
-  if (recorded) return;
-  OXB_CUDA(cudaEventRecord(enqueued_ev_, stream));
-  OXB_CUDA(cudaStreamGetId(stream, &enqueued_on_));
-  enqueued_ = true;
+  if (!recorded) end_enqueued(stream);
 }
 
 void Session::run_wait() {

@@ -208,10 +208,13 @@ class Session {
   void require_not_typed(const std::string& name) const;
   void run_steps(bool profile, bool lanes_wanted, cudaStream_t stream);
   // Runs on callers' streams: the last one's end, which any other stream waits for before it touches the session's memory.
-  cudaEvent_t enqueued_ev_ = nullptr;
+  cudaEvent_t enqueued_ev_ = nullptr, own_ev_ = nullptr;
   unsigned long long enqueued_on_ = 0;  // id of its stream
   bool enqueued_ = false;
-  void follow_enqueued(cudaStream_t s, cudaStream_t also = nullptr);
+  bool own_open_ = false;  // the context's stream may hold work of this session that nobody has waited for
+  void begin_own_work(cudaStream_t also = nullptr);
+  void follow_earlier_runs(cudaStream_t s);
+  void end_enqueued(cudaStream_t s);
   void unbind_inputs();
   void reset_after_error();
   std::vector<DeviceBuffer> arrival_counts_;  // of the kernels whose parts are joined by the last to come; zero between runs

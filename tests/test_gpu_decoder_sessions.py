@@ -11,6 +11,7 @@ import pytest
 
 import decoder_oracle as D
 import test_gpu_decoder as G
+from oxionnx_b200 import _ffi
 from oxionnx_b200.graph import Graph, Node
 from oxionnx_b200.session import Declined, OnnxError, Session
 
@@ -146,3 +147,110 @@ def test_a_run_that_gave_up_leaves_no_counts_of_parts(session_state, way):
     torch.cuda.synchronize()
     assert int(words.count_nonzero()) == 0, "counts of parts are left behind"
     assert np.array_equal(s.run(feeds)["out"], want)
+
+
+# ---- the order of one session's runs ---------------------------------------------------------------
+def refused_calls(s):
+    """Calls that the library refuses after it has begun them."""
+    lib, h = _ffi.lib(), s.ctx.handle
+    fetches = (_ffi.Result * 1)()
+
+    def submit_nothing():
+        return lib.oxb200_run_submit(h, None, 0)
+
+    def run_nothing():
+        return lib.oxb200_run(h, None, 0, fetches, 1)
+
+    def fetch_nothing():
+        return lib.oxb200_fetch_value(h, b"query", ctypes.byref(_ffi.Result(lanes=(ctypes.c_float * 1)(), cap=1)))
+
+    def bound_without_a_feed():
+        return lib.oxb200_run_bound(h, None, 0, fetches, 1)
+
+    return {"run": run_nothing, "submit": submit_nothing, "fetch": fetch_nothing, "bound": bound_without_a_feed}
+
+
+@pytest.mark.parametrize("call", ["run", "submit", "fetch", "bound", "upload"])
+def test_a_refused_call_between_two_enqueued_runs_leaves_their_order(call):
+    """A run behind 100 ms of sleep on one stream, a call that is refused, a run on another stream: the second run ends after
+    the first."""
+    p = D.Paged([1, 90], [50, 90], 4, 2, 64, 16, "float16", seed=86)
+    p.kc, p.vc = torch.nan_to_num(p.kc), torch.nan_to_num(p.vc)
+    s, dev, out = G.check_attend(p)
+    want = out.clone()
+    feeds = host_feeds(dev)
+    calls = refused_calls(s)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    first, second = torch.cuda.Event(), torch.cuda.Event()
+    for _ in range(2):
+        out.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            torch.cuda._sleep(200_000_000)
+        s.enqueue(one.cuda_stream)
+        first.record(one)
+        if call == "upload":  # its copies have begun when the last feed turns out to be missing
+            lib = _ffi.lib()
+            ops, keep = (_ffi.Operand * (len(feeds) - 1))(), _ffi.Keep()
+            names = list(feeds)[:-1]
+            for op, n in zip(ops, names):
+                code = _ffi.dtype_code(s._input_types[n])
+                _ffi.pack_operand(op, n, _ffi.lanes_of(feeds[n], code), keep, dtype=code)
+            assert lib.oxb200_upload_feeds(s.ctx.handle, ops, len(names)) == _ffi.FAILED
+        elif call == "bound":
+            s.clear_bindings()
+            assert calls[call]() == _ffi.FAILED
+            for n, t in dev.items():
+                s.bind_input_device(n, t.data_ptr(), G.name_of(t), t.numel())
+            s.bind_output_device("out", out.data_ptr(), out.numel(), "float16")
+        else:
+            assert calls[call]() == _ffi.FAILED
+        s.enqueue(two.cuda_stream)
+        second.record(two)
+        second.synchronize()
+        assert first.query(), "the second run did not wait for the first"
+        s.wait()
+        assert torch.equal(out, want)
+
+
+def test_a_run_that_failed_half_way_is_waited_for(session_state):
+    """A launch that fails behind others: what is in the stream of that run still comes before the next one."""
+    p = D.Paged([1, 90], [50, 90], 4, 2, 64, 16, "float16", seed=87)
+    s, dev, out = G.check_attend(p)
+    want = out.clone()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    first, second = torch.cuda.Event(), torch.cuda.Event()
+    out.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(one):
+        torch.cuda._sleep(200_000_000)
+    session_state.add_failing_step(s.ctx.handle)
+    with pytest.raises(OnnxError, match="a step that fails"):
+        s.enqueue(one.cuda_stream)
+    session_state.drop_last_step(s.ctx.handle)
+    first.record(one)
+    s.enqueue(two.cuda_stream)
+    second.record(two)
+    second.synchronize()
+    assert first.query(), "the second run did not wait for what the failed one had launched"
+    s.wait()
+    assert torch.equal(out, want)
+
+
+def test_host_runs_then_enqueued_ones():
+    """run and the pipelined form end before they return; a run enqueued behind them reads its own inputs."""
+    p = D.Paged([1, 90], [50, 90], 4, 2, 64, 16, "float16", seed=88)
+    p.kc, p.vc = torch.nan_to_num(p.kc), torch.nan_to_num(p.vc)
+    s, dev, out = G.check_attend(p)
+    want = out.clone()
+    feeds = host_feeds(dev)
+    feeds["query"] = feeds["query"] * 0.5
+    half = s.run(feeds)["out"]
+    stream = torch.cuda.Stream()
+    for _ in range(5):
+        assert np.array_equal(s.run(feeds)["out"], half)
+        s.enqueue(stream.cuda_stream)
+        assert all(np.array_equal(r["out"], half) for r in s.run_pipelined([feeds] * 3))
+        s.enqueue(stream.cuda_stream)
+        s.wait()
+        assert torch.equal(out, want)
