@@ -337,7 +337,8 @@ int oxb200_bind_output_device(oxb200_ctx* ctx, const char* name, void* device_pt
 /* bind_output_device in the output's own element type (`dtype`, the type the graph gives it: f16 and bf16 outputs of the
  * decoder operators, f32 otherwise): the lanes go to `device_ptr` alone, and where nobody fetches them no f32 copy is made.
  * 16-byte aligned buffers that share no memory with another bound buffer are written in place.  While an output is bound so,
- * output_device_ptr and fetch_value refuse it.
+ * output_device_ptr and fetch_value refuse it, and so do they and download_fetches once it is unbound, until a run has made
+ * its f32 lanes.
  *   run_enqueue         run_bound without its fence, on `cuda_stream` (a cudaStream_t of the context's device, NULL: the
  *                       default stream): every input must be bound, nothing is fetched, and the call returns when the
  *                       launches are in the stream.  Bound buffers follow that stream's order like any kernel's operands.

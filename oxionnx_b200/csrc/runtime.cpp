@@ -683,6 +683,11 @@ bool Session::replay_graph(bool lanes_wanted, cudaStream_t stream) {
   return true;
 }
 
+void Session::run_steps(bool profile, bool lanes_wanted) {
+  note_lanes(lanes_wanted, false);
+  run_steps(profile, lanes_wanted, nullptr);
+}
+
 void Session::run_steps(bool profile, bool lanes_wanted, cudaStream_t s) {
   const bool on_own_stream = s == nullptr;
   if (on_own_stream) {
@@ -745,6 +750,7 @@ void Session::download_async(oxb200_result* fetches, uint32_t n) {
   // (write_node_outputs, root crate src/session/run/dispatch.rs:335-455)
   for (uint32_t i = 0; i < n; ++i) {
     const Value& v = values_[output_staging_[i].second];
+    if (fetches[i].lanes) require_lanes(i);
     if (fetches[i].lanes && fetches[i].cap < (uint64_t)v.numel())
       raise(OXB200_FAILED, "run: fetch buffer for '%s' holds %llu lanes, %lld needed", outputs_[i].c_str(), (unsigned long long)fetches[i].cap, (long long)v.numel());
   }
@@ -1042,11 +1048,30 @@ void Session::restore_outputs() {
     }
 }
 
-// The f32 lanes of an output that the last runs wrote to a caller's buffer are not here.
+// Which outputs' f32 lanes a run does not make: those it leaves in the caller's buffer.  A recorded run (`recorded`) makes none
+// before it is replayed.
+void Session::note_lanes(bool lanes_wanted, bool recorded) {
+  lanes_missing_.resize(outputs_.size(), 0);
+  for (size_t i = 0; i < outputs_.size(); ++i) {
+    auto b = bound_out_.find((int)i);
+    const bool missing = !lanes_wanted && b != bound_out_.end() && b->second.typed && (output_raw_[i] >= 0 || b->second.own);
+    lanes_missing_[i] = missing || (recorded && lanes_missing_[i]);
+  }
+}
+
+void Session::require_lanes(size_t output) const {
+  if (output < lanes_missing_.size() && lanes_missing_[output])
+    raise(OXB200_FAILED, "the last run left '%s' in a caller's device buffer in its own type; its f32 lanes were not made", outputs_[output].c_str());
+}
+
+// An output that is bound in its own type is read there, and one whose last run was so has no f32 lanes.
 void Session::require_not_typed(const std::string& name) const {
-  for (const auto& kv : bound_out_)
-    if (kv.second.typed && output_staging_[kv.first].first == name)
-      raise(OXB200_FAILED, "'%s' is bound to a device buffer in its own type; read it there", name.c_str());
+  for (size_t i = 0; i < output_staging_.size(); ++i) {
+    if (output_staging_[i].first != name) continue;
+    auto b = bound_out_.find((int)i);
+    if (b != bound_out_.end() && b->second.typed) raise(OXB200_FAILED, "'%s' is bound to a device buffer in its own type; read it there", name.c_str());
+    require_lanes(i);
+  }
 }
 
 void Session::output_device_ptr(const std::string& name, void** ptr, uint64_t* len) {
@@ -1120,6 +1145,7 @@ void Session::enqueue(cudaStream_t stream) {
   try {
     apply_input_bindings(stream);
     point_outputs();
+    note_lanes(false, recorded);
     run_steps(false, false, stream);
     copy_outputs(stream);
   } catch (...) {

@@ -128,7 +128,7 @@ class Session {
             const std::map<std::string, const HostTensor*>& volatile_consts, const std::vector<std::string>& outputs);
   void upload(const oxb200_operand* feeds, uint32_t n);
   // `lanes_wanted` false: outputs bound in their own type need no f32 lanes.
-  void run_steps(bool profile, bool lanes_wanted = true) { run_steps(profile, lanes_wanted, nullptr); }
+  void run_steps(bool profile, bool lanes_wanted = true);
   // One run of a session whose inputs are all bound, on the caller's stream and without a fence; run_wait() is the fence.
   void enqueue(cudaStream_t stream);
   void run_wait();
@@ -205,6 +205,9 @@ class Session {
   void restore_outputs();
   void copy_outputs(cudaStream_t s);
   bool overlaps_own_memory(const void* p, size_t bytes) const;
+  std::vector<char> lanes_missing_;  // per graph output: the last run made no f32 lanes of it
+  void note_lanes(bool lanes_wanted, bool recorded);
+  void require_lanes(size_t output) const;
   void require_not_typed(const std::string& name) const;
   void run_steps(bool profile, bool lanes_wanted, cudaStream_t stream);
   // Runs on callers' streams: the last one's end, which any other stream waits for before it touches the session's memory.

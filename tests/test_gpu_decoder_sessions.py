@@ -254,3 +254,50 @@ def test_host_runs_then_enqueued_ones():
         s.enqueue(stream.cuda_stream)
         s.wait()
         assert torch.equal(out, want)
+
+
+# ---- f32 lanes of outputs that a run left in the caller's buffer -----------------------------------
+def test_lanes_that_the_last_run_did_not_make_are_not_handed_out():
+    p = D.Paged([1, 90], [50, 90], 4, 2, 64, 16, "float16", seed=84)
+    s, dev, out = G.check_attend(p)  # enqueued with `out` bound in its own type: f32 lanes were never made
+    for call in (s.download, lambda: s.output_device_ptr("out"), lambda: s.fetch_value("out")):
+        with pytest.raises(OnnxError, match="own type"):
+            call()
+    s.clear_bindings()
+    for call in (s.download, lambda: s.output_device_ptr("out"), lambda: s.fetch_value("out")):
+        with pytest.raises(OnnxError, match="own type"):
+            call()
+    for n, t in dev.items():
+        s.bind_input_device(n, t.data_ptr(), G.name_of(t), t.numel())
+    want = out.float().cpu().numpy()
+    assert np.array_equal(s.run_with_binding()["out"], want)  # makes them
+    assert np.array_equal(s.download()["out"], want) and np.array_equal(s.fetch_value("out"), want) and s.output_device_ptr("out")[1] == want.size
+    # the pipelined form makes its own, and a bound run without fetches leaves them out again
+    s.bind_output_device("out", out.data_ptr(), out.numel(), "float16")
+    p2 = dev["query"].clone()
+    dev["query"].mul_(0.5)
+    s.run_with_binding(fetch=False)
+    dev["query"].copy_(p2)
+    s.clear_bindings()
+    with pytest.raises(OnnxError, match="own type"):
+        s.download()
+
+
+def test_one_output_in_its_own_type_beside_one_in_f32():
+    """Only what the run left out is refused."""
+    g = torch.Generator().manual_seed(85)
+    w = D.linear_weights(g, 64, 64, 32, False, False)
+    x = torch.randn(4, 64, generator=g).half().cuda()
+    y, z = torch.empty(4, 64, dtype=torch.float16, device="cuda"), torch.empty(4, 64, device="cuda")
+    s = G.session([G.linear_node(64, 64, 32, w, "y"), ("Add", "s", ["y", "x"], ["z"], {})], {"x": x}, {"y": y, "z": z}, w)
+    s.bind_output_device("z", z.data_ptr(), z.numel())
+    G.run(s)
+    s.clear_bindings()
+    assert np.array_equal(s.fetch_value("z"), z.cpu().numpy())
+    with pytest.raises(OnnxError, match="own type"):
+        s.output_device_ptr("y")
+    s.bind_input_device("x", x.data_ptr(), "float16", x.numel())
+    s.enqueue(0)
+    s.wait()
+    got = s.download()
+    assert np.array_equal(got["y"], y.float().cpu().numpy()) and np.array_equal(got["z"], z.cpu().numpy())
