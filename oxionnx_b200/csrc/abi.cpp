@@ -438,7 +438,7 @@ int oxb200_dispatch(oxb200_ctx* ctx, const oxb200_node* node, const oxb200_opera
         if (v->bytes) OXB_CUDA(cudaMemcpyAsync(t->h.ptr, v->ptr, v->bytes, cudaMemcpyDeviceToDevice, C.stream()));
         sess.sync();
         const int flag = sess.check_error_flag();
-        if (flag) raise(OXB200_FAILED, flag == 20 ? "Gather: an index is out of range (device code %d)" : "a tensor-core kernel gave up on a bounded wait (code %d)", flag);
+        if (flag) raise(OXB200_FAILED, error_text(flag), flag);
       } catch (...) {
         C.give_block(t->h.ptr, t->h.bytes);
         throw;
@@ -811,7 +811,7 @@ int oxb200_run_resident(oxb200_ctx* ctx, uint32_t iters, float* elapsed_ms) {
           if (cudaEventElapsedTime(&t, st.ev0, st.ev1) == cudaSuccess) st.last_ms = t;
         }
     int flag = s.check_error_flag();
-    if (flag) raise(OXB200_FAILED, flag == 20 ? "Gather: an index is out of range (device code %d); results are not valid" : "a tensor-core kernel gave up on a bounded wait (code %d); results are not valid", flag);
+    if (flag) raise(OXB200_FAILED, error_text(flag), flag);
     return (int)OXB200_OK_DEVICE;
   });
 }

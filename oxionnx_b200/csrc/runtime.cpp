@@ -727,7 +727,7 @@ void Session::download(oxb200_result* fetches, uint32_t n) {
 }
 
 // What the kernels' error word says; every text takes the code.
-static const char* error_text(int flag) {
+const char* error_text(int flag) {
   switch (flag) {
     case 20: return "Gather: an index is out of range (device code %d); results are not valid";
     case 21: return "paged cache: an entry of the page table that a sequence needs is no page of the cache (device code %d); what needed it was skipped";
@@ -922,7 +922,8 @@ void Session::collect(oxb200_result* fetches, uint32_t n) {
     OXB_CUDA(cudaStreamSynchronize(down_stream_));
     if (other.busy) other.poisoned = true;
     reset_after_error();
-    raise(OXB200_FAILED, "a kernel reported code %d during a pipelined run (or the run before it failed while this one was in flight); results are not valid", flag);
+    if (flag == 0) raise(OXB200_FAILED, "collect: the run before this one failed while it was in flight; results are not valid");
+    raise(OXB200_FAILED, error_text(flag), flag);
   }
   for (uint32_t i = 0; i < n; ++i) {
     const Value& v = values_[output_staging_[i].second];

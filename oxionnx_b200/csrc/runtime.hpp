@@ -118,6 +118,9 @@ struct DeviceBuffer {
 
 class Context;
 
+// What a code of the kernels' error word says; every text takes the code.
+const char* error_text(int flag);
+
 // One planned graph (a whole session, or the one-node graph of a dispatch).
 class Session {
  public:

@@ -301,3 +301,23 @@ def test_one_output_in_its_own_type_beside_one_in_f32():
     s.wait()
     got = s.download()
     assert np.array_equal(got["y"], y.float().cpu().numpy()) and np.array_equal(got["z"], z.cpu().numpy())
+
+
+# ---- what the error word says --------------------------------------------------------------------
+def test_every_call_that_waits_says_what_is_wrong():
+    p = D.Paged([1, 1], [40, 30], 4, 2, 64, 16, "float16", seed=83)
+    p.kc, p.vc = torch.nan_to_num(p.kc), torch.nan_to_num(p.vc)
+    s, dev, out = G.check_attend(p)
+    good = host_feeds(dev)
+    for change, match in (({"page_table": np.full_like(good["page_table"], 10_000)}, "page table"), ({"cu_query": np.array([0, 2, 1], np.int32)}, "cu_query"),
+                          ({"cu_query": np.array([0, 0, 2], np.int32)}, "max_query_length")):
+        bad = {**good, **change}
+        with pytest.raises(OnnxError, match=match):
+            s.run(bad)
+        s.upload(bad)
+        with pytest.raises(OnnxError, match=match):
+            s.run_resident(1)
+        s.submit(bad)
+        with pytest.raises(OnnxError, match=match):
+            s.collect()
+        assert np.array_equal(s.run(good)["out"], out.float().cpu().numpy())
