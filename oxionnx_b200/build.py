@@ -31,7 +31,7 @@ OBJECTS = {
 }
 # headers of the decoder operators, which nothing but these objects includes
 DECODER_HEADERS = ["decoder.hpp", "decoder_device.cuh", "decoder_schedule.hpp"]
-DECODER_OBJECTS = ("planner", "paged_append", "paged_attention", "umma_prompt", "linear4", "umma_linear4")
+DECODER_OBJECTS = ("planner", "runtime", "paged_append", "paged_attention", "umma_prompt", "linear4", "umma_linear4")
 HEADERS = ["common.hpp", "kernels.hpp", "runtime.hpp", "umma_kernel.cuh", "umma_epilogue8.cuh", "umma_launch.cuh", "umma_small.cuh", "pdl.cuh", "umma_chain.cuh", "model.hpp", "abi_internal.hpp", os.path.join("..", "..", "include", "oxb200.h")]
 
 

@@ -20,8 +20,8 @@ struct PagedTables {
   int64_t tokens;  // rows of the packed queries
 };
 
-// Codes of the error word (see error_text in runtime.cpp).
-constexpr int kErrPage = 21, kErrPosition = 22, kErrLengths = 23, kErrQueryLength = 24;
+// Codes of the error word (see error_text in runtime.cpp), none of which a wait of another kernel has.
+constexpr int kErrPage = 71, kErrPosition = 72, kErrLengths = 73, kErrQueryLength = 74;
 constexpr int kMaxSequences = 4096;
 
 struct PagedAppend {

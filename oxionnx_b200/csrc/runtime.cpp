@@ -1,5 +1,6 @@
 // Context, weight residency, arena planning and the run loop of the oxb200 provider.
 // The per-operator planning rules live in planner.cpp.
+#include "decoder.hpp"
 #include "runtime.hpp"
 
 #include <algorithm>
@@ -730,10 +731,10 @@ void Session::download(oxb200_result* fetches, uint32_t n) {
 const char* error_text(int flag) {
   switch (flag) {
     case 20: return "Gather: an index is out of range (device code %d); results are not valid";
-    case 21: return "paged cache: an entry of the page table that a sequence needs is no page of the cache (device code %d); what needed it was skipped";
-    case 22: return "paged cache: a token's position has no row in cos / sin (device code %d); the token was skipped";
-    case 23: return "paged cache: cu_query does not rise from 0 to the number of query rows, or a length exceeds the page table (device code %d); results are not valid";
-    case 24: return "OxiPagedAttention: a sequence has more query rows than max_query_length (device code %d); results are not valid";
+    case k::kErrPage: return "paged cache: an entry of the page table that a sequence needs is no page of the cache (device code %d); what needed it was skipped";
+    case k::kErrPosition: return "paged cache: a token's position has no row in cos / sin (device code %d); the token was skipped";
+    case k::kErrLengths: return "paged cache: cu_query does not rise from 0 to the number of query rows, or a length exceeds the page table (device code %d); results are not valid";
+    case k::kErrQueryLength: return "OxiPagedAttention: a sequence has more query rows than max_query_length (device code %d); results are not valid";
     default: return "a tensor-core kernel gave up on a bounded wait (code %d); results are not valid";
   }
 }

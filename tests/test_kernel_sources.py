@@ -46,3 +46,16 @@ def test_blocks_that_others_read_from_leave_together():
         depth = body[: barriers[-1]].count("{") - body[: barriers[-1]].count("}")
         assert depth <= 1, f"{source}: the last barrier of the cluster stands inside of {depth} blocks"
     assert "if (clustered) cluster_sync_all();" in dict(functions("umma_chain.cu"))["umma_chain_kernel"]
+
+
+def test_codes_of_the_error_word_say_one_thing():
+    """The codes that have a text of their own are no kernel's code of a wait that ran out."""
+    with open(os.path.join(CSRC, "decoder.hpp")) as fh:
+        named = {int(c) for c in re.findall(r"kErr\w+ = (\d+)", fh.read())}
+    assert len(named) == 4
+    waits = set()
+    for source in SOURCES:
+        for _, body in functions(source):
+            waits |= {int(c) for c in re.findall(r"(?:give_up\(|fail\(abortp, p\.err_flag, |atomicExch\([^;]*?err[^;]*?, )(\d+)\)", body)}
+            waits |= {int(c) for c in re.findall(r"wait\(bar_\w+(?:\[[^;]*?\])?, [^;]*?, (\d+)\)", body)}
+    assert len(waits) > 15 and not waits & named, sorted(waits & named)
