@@ -162,7 +162,10 @@ typedef struct {
  *            index; optional bias [N].  All but x are initializers.
  *   attrs    K, N, bits = 4, block_size (a power of two, 16 .. 1024)
  *   output   [.., N] in x's type.  Sums are f32.  17 rows and more of 16 bits multiply weights that are rounded once to x's
- *            type; fewer, and f32 rows, exact ones.
+ *            type; fewer, and f32 rows, exact ones.  The rounding is half a step of the weight whatever the scale: powers of two
+ *            are taken out of an output's scales where its weights would overflow x's type or leave its normal numbers, and a
+ *            matrix with scales of one output further apart than the type's normal numbers is multiplied exactly, at the
+ *            fewer rows' rate.
  *
  * The paged operators share five inputs.  A cache is [pages][page][kv_heads][size], 16-bit, pages of a multiple of 16 tokens,
  * heads of a multiple of 8 lanes up to 256.  cu_query i32 [sequences + 1]: the new rows' bounds, from 0 up.  Rows behind the

@@ -2,6 +2,8 @@
 // enqueues on a stream, never synchronises.
 #pragma once
 
+#include <vector>
+
 #include "common.hpp"
 
 namespace oxb {
@@ -68,6 +70,8 @@ struct Linear4 {
   const void* scales;
   const uint8_t* zeros;   // null: 8
   bool scales_f16;        // scales are f16, f32 otherwise
+  const float* unfold;    // [n]: what the sums of an output are multiplied by, powers of two; null: nothing
+  bool exact_weights;     // 16-bit rows: their weights may not be rounded, however many rows there are
   const float* bias;      // null: none
   int64_t rows;
   int k, n, group, groups;  // groups: of one output's inputs, the last one perhaps short
@@ -75,6 +79,9 @@ struct Linear4 {
   void* workspace;          // linear4_workspace bytes, or null
   int* err;
 };
+// Powers of two by which each output's scales [n][groups] are multiplied before the weights are rounded to x's type, so that none
+// overflows or loses bits (empty: all 0).  False where there are none, and the weights must not be rounded.
+bool linear4_folds(const Linear4& a, const float* scales, bool zero_points, std::vector<int>* folds);
 size_t linear4_workspace(const Linear4& a);
 void linear4(const Linear4& a, cudaStream_t s);
 bool linear4_many_rows(const Linear4& a);

@@ -545,7 +545,8 @@ void launch_rows(const Linear4& a, cudaStream_t s) {
     const int64_t rows = std::min<int64_t>(a.rows - row0, 65535LL * 16);
     if (rows <= 8) large ? launch_rows<T, 4, 1>(a, row0, rows, s) : launch_rows<T, 1, 1>(a, row0, rows, s);
     else if (rows <= 16 || sizeof(T) == 4) large ? a.n >= 64 * 148 ? launch_rows<T, 4, 2>(a, row0, rows, s) : launch_rows<T, 2, 2>(a, row0, rows, s) : launch_rows<T, 1, 2>(a, row0, rows, s);
-    else launch_rows<T, 1, 4>(a, row0, rows, s);
+    else if constexpr (sizeof(T) == 2) launch_rows<T, 1, 4>(a, row0, rows, s);  // of exact weights
+
   }
 }
 
@@ -555,7 +556,7 @@ void launch_rows(const Linear4& a, cudaStream_t s) {
 // against that one, at 4096x4096: 16 rows 7.2 / 9.8 us, 32 rows 13.0 / 10.2, 64 rows 24.9 / 10.4.
 constexpr int64_t kManyRows = 17;
 
-bool linear4_many_rows(const Linear4& a) { return a.dt != DT::F32 && a.rows >= kManyRows; }
+bool linear4_many_rows(const Linear4& a) { return a.dt != DT::F32 && a.rows >= kManyRows && !a.exact_weights; }
 
 void linear4(const Linear4& a, cudaStream_t s) {
   if (a.rows == 0) return;

@@ -3132,13 +3132,24 @@ void Planner::plan_matmul_4bit(const NodeDef& n) {
   a.codes = C.resident_form(in_name(n, 1), shape, (size_t)Layout4::code_bytes(N, K),
                             [&](void* p) { Layout4::codes(codes->data.data(), N, K, group, (uint8_t*)p); }, cacheable_const(in_name(n, 1)));
   // scales keep their 16 bits where f16 holds them, as it does those of a model that stores them so
-  const int64_t lanes = Layout4::tiles(N) * groups * 16;
   a.scales_f16 = true;
   for (float v : scales->data) a.scales_f16 = a.scales_f16 && __half2float(__float2half_rn(v)) == v;
-  a.scales = C.resident_form(in_name(n, 2), shape, (size_t)lanes * (a.scales_f16 ? 2 : 4), [&](void* p) {
+  std::vector<int> folds;  // where weights are rounded to x's type: powers of two that bring an output's scales into its range
+  if (k::linear4_many_rows(a)) a.exact_weights = !k::linear4_folds(a, scales->data.data(), zeros != nullptr, &folds);
+  std::string scales_form = shape;
+  if (!folds.empty()) {
+    a.scales_f16 = false;
+    const std::string how = std::string(" folded for ") + dt_name(a.dt) + (zeros ? " 15" : " 8");
+    scales_form += how;
+    a.unfold = (const float*)C.resident_form(in_name(n, 2), shape + " unfold" + how, (size_t)N * 4, [&](void* p) {
+      for (int64_t o = 0; o < N; ++o) ((float*)p)[o] = (float)std::ldexp(1.0, -folds[o]);
+    }, cacheable_const(in_name(n, 2)));
+  }
+  const int64_t lanes = Layout4::tiles(N) * groups * 16;
+  a.scales = C.resident_form(in_name(n, 2), scales_form, (size_t)lanes * (a.scales_f16 ? 2 : 4), [&](void* p) {
     for (int64_t o = 0; o < N; ++o)
       for (int64_t g = 0; g < groups; ++g) {
-        const float v = scales->data[o * groups + g];
+        const float v = folds.empty() ? scales->data[o * groups + g] : std::ldexp(scales->data[o * groups + g], folds[o]);
         if (a.scales_f16) ((__half*)p)[Layout4::of_group(o, g, groups)] = __float2half_rn(v);
         else ((float*)p)[Layout4::of_group(o, g, groups)] = v;
       }

@@ -8,13 +8,17 @@
 // of 64 inputs by 256 rows take 512 cycles.  With eight warps a block of inputs took 800, as long as one's decoding; with
 // sixteen 650: 2048 x 4096 x 4096 takes 62 us, 1110 TFLOP/s, in two turns of 256 tiles over 148 SMs.
 //
-// The roundings of the weights are as large as those of the result (half a step of x's type each, and independent).
+// The roundings of the weights are as large as those of the result (half a step of x's type each, and independent).  For that
+// they have to be normal numbers of x's type: outputs with scales that would leave it bring a power of two with them, which
+// the sums are multiplied by in the end (linear4_folds).
 // Every wait is bounded.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "decoder_device.cuh"
 #include "umma_kernel.cuh"
@@ -265,6 +269,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
       tc_fence_after();
       const int out = out0 + r;
       const float bias = a.bias && out < a.n ? a.bias[out] : 0.f;
+      const float unfold = a.unfold && out < a.n ? a.unfold[out] : 1.f;
       uint8_t* const staging = base_ptr + turn * 8192;  // 32 rows of 128 outputs
       const int outs = min(L4_OUTPUTS, a.n - out0);
       const bool wide = a.n % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
@@ -280,7 +285,7 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
           continue;
         }
 #pragma unroll
-        for (int e = 0; e < 32; ++e) *(T*)(staging + e * 256 + r * 2) = from_f32<T>(__uint_as_float(v[e]) + bias);
+        for (int e = 0; e < 32; ++e) *(T*)(staging + e * 256 + r * 2) = from_f32<T>(__uint_as_float(v[e]) * unfold + bias);
         asm volatile("bar.sync %0, 128;" ::"r"(1 + turn) : "memory");
         const int i = (int)threadIdx.x & 127;
         if (wide) {
@@ -316,7 +321,10 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
       T out[4];
       const float v[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = from_f32<T>(a.bias && col + e < outs ? v[e] + a.bias[out0 + col + e] : v[e]);
+      for (int e = 0; e < 4; ++e) {
+        const float y = a.unfold && col + e < outs ? v[e] * a.unfold[out0 + col + e] : v[e];
+        out[e] = from_f32<T>(a.bias && col + e < outs ? y + a.bias[out0 + col + e] : y);
+      }
       T* const to = (T*)a.y + (row0 + row) * a.n + out0 + col;
       if (wide) *(uint2*)to = *(const uint2*)out;
       else
@@ -446,6 +454,33 @@ void launch_prompt(const Linear4& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+// A weight (code - zero) * scale is normal in x's type from its least normal number up, and finite up to its largest; products with
+// f16 scales of any size are exact below f16's normal numbers.  An output that has scales outside of that gets the power of two
+// that puts its largest scale at 2^11 (f16: 15 times it still fits) or 1 (bf16), from where 25 (126) powers of two lie above the
+// least normal number.
+bool linear4_folds(const Linear4& a, const float* scales, bool zero_points, std::vector<int>* folds) {
+  const bool f16 = a.dt == DT::F16;
+  const double most = f16 ? 65504.0 : 0x1.fep127, least = f16 ? 0x1p-14 : 0x1p-126, reach = zero_points ? 15.0 : 8.0;
+  std::vector<int> out((size_t)a.n, 0);
+  bool any = false;
+  for (int64_t n = 0; n < a.n; ++n) {
+    double high = 0.0, low = HUGE_VAL;
+    for (int g = 0; g < a.groups; ++g) {
+      const double v = std::fabs((double)scales[n * a.groups + g]);
+      if (!std::isfinite(v)) return false;  // it is the sum of its group that is multiplied by it
+      high = std::max(high, v);
+      if (v > 0.0) low = std::min(low, v);
+    }
+    if (high * reach <= most && (low >= least || a.scales_f16)) continue;
+    const int fold = (f16 ? 11 : 0) - std::ilogb(high);
+    if (std::ldexp(low, fold) < least) return false;
+    out[n] = fold;
+    any = true;
+  }
+  if (any) folds->swap(out);
+  return true;
+}
 
 // Rows that TMA does not take as they lie (their length no multiple of 16 bytes) are copied.
 size_t linear4_workspace(const Linear4& a) { return linear4_many_rows(a) && a.k % 8 != 0 ? (size_t)a.rows * ((a.k + 7) / 8 * 8) * 2 : 0; }
