@@ -25,6 +25,10 @@ constexpr int kShortRows = 64;  // packed rows of a sequence up to which it is s
 // than the keys.  4 short streams (12 heads of 64, 700 tokens) with at least 4 / 8 / 16 steps 15.7 / 19.7 / 27.8 us; 64 streams
 // of up to 8100 tokens with 2 / 4 / 8 pieces 195.9 / 196.5 / 197.9.
 constexpr int kBegin = 2, kLeast = 4;
+// A probability is 2^(score slope - maximum slope), one multiplication and addition with the rounded product of the maximum, whose
+// error (2^-24 of it) is a factor of the whole row.  Where the product is above this, parts whose maxima differ would no longer fit
+// together (2^-14 here; from 2^28 on powers of two overflow): there the maximum is taken off the scores first.
+constexpr float kFar = 1024.f;
 
 // Lanes of a head in shared memory (zeros behind its own), warps of a block and stages of a warp's ring.  A warp streams a piece
 // of keys and one of values a stage through cp.async and keeps its own maximum, sum and accumulator.
@@ -308,6 +312,8 @@ __global__ void __launch_bounds__(Shape<KD>::kWarps * 32, 1) paged_attention_sho
 #pragma unroll
           for (int e = 0; e < 4; ++e) qf[k][e] ^= flip;
       most[0] = most[1] = -INFINITY, sum[0] = sum[1] = 0.f;
+      float bias[2] = {0.f, 0.f};  // what is taken off scaled scores
+      bool far = false;            // a maximum is far from 0: it is taken off the scores before they are scaled
 #pragma unroll
       for (int n = 0; n < KD / 8; ++n)
 #pragma unroll
@@ -352,7 +358,7 @@ __global__ void __launch_bounds__(Shape<KD>::kWarps * 32, 1) paged_attention_sho
           top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
           top[h] = fmaxf(top[h], most[h]);
         }
-        if (__any_sync(0xffffffffu, top[0] > most[0] || top[1] > most[1])) {
+        if (far || __any_sync(0xffffffffu, top[0] > most[0] || top[1] > most[1])) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float keep = most[h] == -INFINITY ? 0.f : exp2_approx((most[h] - top[h]) * slope);
@@ -360,9 +366,19 @@ __global__ void __launch_bounds__(Shape<KD>::kWarps * 32, 1) paged_attention_sho
             sum[h] *= keep;
 #pragma unroll
             for (int n = 0; n < KD / 8; ++n) acc[n][2 * h] *= keep, acc[n][2 * h + 1] *= keep;
+            bias[h] = most[h] == -INFINITY ? 0.f : most[h] * slope;
+          }
+          far = __any_sync(0xffffffffu, fabsf(bias[0]) > kFar || fabsf(bias[1]) > kFar);
+          if (far) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (most[h] == -INFINITY) continue;  // so are the scores
+              bias[h] = 0.f;
+#pragma unroll
+              for (int n = 0; n < 2; ++n) s[n][2 * h] -= most[h], s[n][2 * h + 1] -= most[h];
+            }
           }
         }
-        const float bias[2] = {most[0] == -INFINITY ? 0.f : most[0] * slope, most[1] == -INFINITY ? 0.f : most[1] * slope};
         uint32_t p[4];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
