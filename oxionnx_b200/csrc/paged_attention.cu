@@ -77,6 +77,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// log2 of what the largest probability of a row is written as.  Probabilities are rounded to 16 bits for their product with the
+// values, and the many small ones of a long past may be all that an output is made of: in f16, whose normal numbers end at 2^-14,
+// the largest is 2^15, so that they go down to 2^-29 of it; bf16 has f32's range.  The sums are as much larger and take it out.
+template <typename T>
+constexpr float kLift = 0.f;
+template <>
+constexpr float kLift<__half> = 15.f;
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, __half*) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *(const uint32_t*)&h;
@@ -366,14 +373,14 @@ __global__ void __launch_bounds__(Shape<KD>::kWarps * 32, 1) paged_attention_sho
             sum[h] *= keep;
 #pragma unroll
             for (int n = 0; n < KD / 8; ++n) acc[n][2 * h] *= keep, acc[n][2 * h + 1] *= keep;
-            bias[h] = most[h] == -INFINITY ? 0.f : most[h] * slope;
+            bias[h] = most[h] == -INFINITY ? 0.f : fmaf(most[h], slope, -kLift<T>);
           }
           far = __any_sync(0xffffffffu, fabsf(bias[0]) > kFar || fabsf(bias[1]) > kFar);
           if (far) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (most[h] == -INFINITY) continue;  // so are the scores
-              bias[h] = 0.f;
+              bias[h] = -kLift<T>;
 #pragma unroll
               for (int n = 0; n < 2; ++n) s[n][2 * h] -= most[h], s[n][2 * h + 1] -= most[h];
             }

@@ -12,8 +12,8 @@
 //
 // The two tiles take turns: while one's scores become probabilities, the other's products run.  A tile's next scores follow
 // its own probabilities' product, since both use its columns of tensor memory.  The output is only rescaled when a row's
-// maximum has grown by more than 2^8 (it is exact arithmetic up to rounding whichever maximum is used; the sums stay in f32
-// and the 16-bit probabilities below 2^8), which after the first tiles is rare.
+// maximum has grown by more than 2^8 (f16: 2^4; it is exact arithmetic up to rounding whichever maximum is used; the sums stay in
+// f32 and the 16-bit probabilities below 2^8, f16's below 2^15), which after the first tiles is rare.
 //
 // One block per SM takes an equal run of all items' key tiles (PromptWork), so that one long prompt, many short ones and a few
 // rows behind a long past fill the chip alike; items run into one another without a pause: the next item's queries are brought
@@ -40,7 +40,16 @@ constexpr int PR_KEYS = 128, PR_ROWS = 128;
 constexpr int PR_THREADS = 384;  // three warpgroups; the last two warps of the third idle
 constexpr int PR_LEAST_STEPS = 6;  // steps that a block takes at least: below, joining the parts costs more than the keys
 constexpr float PR_FAR = 1024.f;  // product of maximum and slope above which the maximum is taken off first (kFar of paged_attention.cu)
-constexpr float PR_GROWTH = 8.f;  // log2 of how far probabilities may exceed 1 before the output is rescaled
+// log2 of what the probability of the maximum is written as (kLift of paged_attention.cu), and of how far others may exceed it before
+// the output is rescaled: together below f16's 2^16.
+template <typename T>
+constexpr float PR_LIFT = 0.f;
+template <>
+constexpr float PR_LIFT<__half> = 11.f;
+template <typename T>
+constexpr float PR_GROWTH = 8.f;
+template <>
+constexpr float PR_GROWTH<__half> = 4.f;
 
 template <int KD>
 struct PromptShape {
@@ -549,8 +558,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
               tmem_st16(o_col + 16 * c, o);
             }
           }
-          bias = top == -INFINITY ? 0.f : -top * p.slope;
-          growth = PR_GROWTH / p.slope;
+          bias = top == -INFINITY ? 0.f : fmaf(-top, p.slope, PR_LIFT<T>);
+          growth = PR_GROWTH<T> / p.slope;
           // Here, where a step seldom comes: a branch of its own in front of the exponentials cost a long prompt 2.5 %.
           if (__any_sync(0xffffffffu, fabsf(bias) > PR_FAR)) {
             if (top != -INFINITY) {  // scores are -infinity with it
@@ -559,7 +568,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
 #pragma unroll
                 for (int e = 0; e < 32; ++e) r[c][e] = __float_as_uint(__uint_as_float(r[c][e]) - top);
             }
-            bias = 0.f, growth = -INFINITY;
+            bias = PR_LIFT<T>, growth = -INFINITY;
           }
         }
         uint64_t part = 0;  // two sums

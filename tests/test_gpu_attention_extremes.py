@@ -1,5 +1,5 @@
-"""OxiPagedAttention where softmax leaves little room: scores of any size.  Queries and keys have one lane that is not 0, so that
-scores are exact and what is expected follows from them alone."""
+"""OxiPagedAttention where softmax leaves little room: scores of any size, and long tails of small probabilities.  Queries and keys
+have one lane that is not 0, so that scores are exact and what is expected follows from them alone."""
 import math
 
 import pytest
@@ -63,3 +63,32 @@ def test_attention_of_scores_of_any_size(kind, query, key, new, total, size, sig
         bound = D.rounding(kind, want) + 2 * D.half_step(kind) * mean + 2 * off + (n + 16) * 2.0**-22 * mean + low_bits
         assert not torch.isnan(got[row]).any(), f"NaN in row {row}"
         assert ((got[row] - want).abs() <= bound).all(), (row, ((got[row] - want).abs() - bound).max())
+
+
+# ---- long tails of small probabilities -----------------------------------------------------------
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("new,total,size", [(1, 40000, 64), (1, 3000, 128), (1, 3000, 256), (3, 40000, 64), (80, 40000, 64), (70, 6000, 128)])
+@pytest.mark.parametrize("gap", [11.0, 17.6, 19.5])
+def test_attention_keeps_what_many_small_probabilities_sum_up_to(new, total, size, gap, kind):
+    """One key takes nearly everything, in a value of 0; the others' exponentials, exp(-gap) each, are all that the output is
+    made of.  Each is rounded to the 16-bit type: half a step, and of f16 below its least normal number 2^-25 of what one is
+    written as.  The kernels write 2^15 (streamed) and 2^11 (tiles) for the largest, so that e^-19.5 = 2^-28.1 loses 2^-36 at
+    most, 0.4 % of it; the f32 sums lose (t + 16) * 2^-22."""
+    p = D.Paged([new], [total], 1, 1, size, 16, kind, seed=91)
+    flat = lambda c: c.view(-1, 1, size)  # noqa: E731
+    slots = torch.tensor([int(p.table[0, j // 16]) * 16 + j % 16 for j in range(total)])
+    flat(p.kc)[slots] = 0
+    flat(p.vc)[slots] = 1
+    at = slots[total // 2]
+    flat(p.kc)[at, 0, 0] = gap / 4  # a 16-bit number: the definition takes it as it is
+    flat(p.vc)[at] = 0
+    p.q[:] = 0
+    p.q[:, 0] = 4
+    s, dev, out = G.check_attend(p, scale=1.0)
+    score = 4 * float(p.kc.view(-1, 1, size)[at, 0, 0])
+    for i in range(new):
+        others = total - new + i
+        tail = others * math.exp(-score)
+        want = torch.full((size,), tail / (1 + tail), dtype=torch.float64)
+        off = 2 * D.half_step(kind) + (2.0**-36 / math.exp(-score) if kind == "float16" else 0) + (total + 16) * 2.0**-22 + 2 * (size + 4) * 2.0**-23 * score
+        G.within(out[i], want, D.rounding(kind, want) + off * want)
