@@ -38,6 +38,7 @@ struct PromptWork {
     const int a = tiles_of(i, 0), b = tiles_of(i, 1), most = a > b ? a : b;
     return most > 0 ? most : 1;
   }
+  OXB_HD int steps(int i) const { return tiles(i) + kBegin; }  // of an item of block i
   // sum of floor((a i + b) / m) over i = 0 .. n - 1, by Euclid's steps on (a, m); a, m up to 2^9, b below 2^32, n below 2^23
   static OXB_HD long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
     long long sum = 0;
@@ -65,15 +66,29 @@ struct PromptWork {
     return (n + (long long)kBegin * (i < all ? i : all)) * kv_heads;
   }
   OXB_HD long long total() const { return rows > 0 ? before(blocks()) : 0; }
-  // the block that step `at` of the sequence lies in
-  OXB_HD int block_at(long long at) const {
-    int lo = 0, hi = blocks() - 1;
-    while (lo < hi) {
-      const int mid = lo + (hi - lo + 1) / 2;
-      if (before(mid) <= at) lo = mid;
-      else hi = mid - 1;
+  // The block that step `inside` of the sequence lies in, 32 blocks at a time; what is left of `inside` is the step within it, all
+  // key heads.  lanes(steps, inside): of 32 lanes with steps(lane) steps each, the first whose end lies behind `inside`, and the
+  // steps of those in front of it; without one, lane 32 and the steps of all.
+  struct Found {
+    int lane;
+    long long before;
+  };
+  template <typename Lanes>
+  OXB_HD int block_of(long long* inside, Lanes&& lanes) const {
+    for (int block = 0;; block += 32) {
+      const Found f = lanes([&](int lane) { return block + lane < blocks() ? (long long)steps(block + lane) * kv_heads : 0LL; }, *inside);
+      *inside -= f.before;
+      if (f.lane < 32) return block + f.lane;
+      if (block + 32 >= blocks()) return blocks() - 1;  // `inside` is no step of the sequence
     }
-    return lo;
+  }
+  // the same on the host, lane by lane
+  OXB_HD int block_at(long long at) const {
+    return block_of(&at, [](auto steps, long long inside) {
+      Found f{0, 0};
+      for (; f.lane < 32 && f.before + steps(f.lane) <= inside; ++f.lane) f.before += steps(f.lane);
+      return f;
+    });
   }
 };
 

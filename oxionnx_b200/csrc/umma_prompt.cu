@@ -107,13 +107,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 // with its wait
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -268,10 +261,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
           if (block < 0) {  // the first item of a sequence (or of this block)
             q = sequence_of(a.t, b, &bad);
             w = work_of(q);
-            // the block that step at - seq_before lies in, 32 at a time (a search by before() took 10 us of divisions)
+            // (a search by before() took 10 us of divisions)
             long long inside = at - seq_before;
-            for (block = 0;; block += 32) {
-              const long long mine = block + lane < w.blocks() ? (long long)(w.tiles(block + lane) + PromptWork::kBegin) * a.kv_heads : 0;
+            block = w.block_of(&inside, [&](auto steps, long long inside) {
+              const long long mine = steps(lane);
               long long sum = mine;
 #pragma unroll
               for (int o = 1; o < 32; o *= 2) {
@@ -279,20 +272,14 @@ __global__ void __launch_bounds__(PR_THREADS, 1) umma_prompt_kernel(const __grid
                 if (lane >= o) sum += up;
               }
               const unsigned in = __ballot_sync(0xffffffffu, sum > inside);
-              if (in || block + 32 >= w.blocks()) {
-                const int who = in ? __ffs(in) - 1 : 31;
-                inside -= __shfl_sync(0xffffffffu, sum - mine, who);
-                block += who;
-                break;
-              }
-              inside -= __shfl_sync(0xffffffffu, sum, 31);
-            }
-            const int steps = w.tiles(block) + PromptWork::kBegin;
+              const int who = in ? __ffs(in) - 1 : 31;
+              return PromptWork::Found{in ? who : 32, __shfl_sync(0xffffffffu, in ? sum - mine : sum, who)};
+            });
+            const int steps = w.steps(block);
             kv = (int)quotient(inside, steps);
             item_at = at - (inside - (long long)kv * steps);
           }
-          const int tiles = w.tiles(block);
-          const long long item_end = item_at + tiles + PromptWork::kBegin, end = min(stop, item_end);
+          const long long item_end = item_at + w.steps(block), end = min(stop, item_end);
           it.j0 = (int)max(0LL, at - item_at - PromptWork::kBegin), it.j1 = (int)(end - item_at - PromptWork::kBegin);
           if (it.j1 > it.j0) {
             it.valid = 1, it.b = b, it.bad = bad ? 1 : 0;
