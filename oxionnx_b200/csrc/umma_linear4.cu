@@ -304,6 +304,21 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
     }
   }
 
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (abort_flag && threadIdx.x == 0) {
+    // give copies that may still be in flight time to land before the block's shared memory goes away
+    const long long start = clock64();
+    while (clock64() - start < 2000000LL) {
+    }
+  }
+  __syncthreads();
+  // In front of the meeting below: on another stream a cluster of the small-product kernel may hold the columns that a block of this
+  // one's waits for while it waits for these.
+  if (warp == 4 * L4_GROUPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_slot), "r"(512) : "memory");
+
   // ---------------- a cluster's sums, in the order of the inputs: every block has its share of the rows ----------------
   if (p.splits > 1) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -334,19 +349,6 @@ __global__ void __launch_bounds__(L4_THREADS, 1) umma_linear4_kernel(const __gri
     }
     cluster.sync();
   }
-
-  // ---------------- teardown ----------------
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  if (abort_flag && threadIdx.x == 0) {
-    // give copies that may still be in flight time to land before the block's shared memory goes away
-    const long long start = clock64();
-    while (clock64() - start < 2000000LL) {
-    }
-  }
-  __syncthreads();
-  if (warp == 4 * L4_GROUPS) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base_slot), "r"(512) : "memory");
 }
 
 // Rows whose length is no multiple of 16 bytes, once more with a stride that is one: 16 bytes a thread.

@@ -322,3 +322,24 @@ def test_every_call_that_waits_says_what_is_wrong():
         with pytest.raises(OnnxError, match=match):
             s.collect()
         assert np.array_equal(s.run(good)["out"], out.float().cpu().numpy())
+
+
+def test_a_linear_and_a_small_product_on_two_streams():
+    """Both run in clusters whose blocks take tensor memory and meet; side by side on the same SMs they end, and give what each
+    gives alone."""
+    g = torch.Generator().manual_seed(89)
+    w = D.linear_weights(g, 1024, 4096, 32, True, False)
+    x, y = torch.randn(64, 4096, generator=g).bfloat16().cuda(), torch.empty(64, 1024, dtype=torch.bfloat16, device="cuda")
+    a = G.session([G.linear_node(4096, 1024, 32, w)], {"x": x}, {"y": y}, w)
+    u, z = torch.randn(256, 2048, generator=g).cuda(), torch.empty(256, 256, device="cuda")
+    b = G.session([("MatMul", "product", ["u", "w"], ["z"], {})], {"u": u}, {"z": z}, {"w": torch.randn(2048, 256, generator=g).numpy()})
+    G.run(a), G.run(b)
+    first, second = y.clone(), z.clone()
+    y.zero_(), z.zero_()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(300):
+        a.enqueue(streams[0].cuda_stream)
+        b.enqueue(streams[1].cuda_stream)
+    a.wait(), b.wait()
+    assert torch.equal(y, first) and torch.equal(z, second)

@@ -48,6 +48,14 @@ def test_blocks_that_others_read_from_leave_together():
     assert "if (clustered) cluster_sync_all();" in dict(functions("umma_chain.cu"))["umma_chain_kernel"]
 
 
+def test_blocks_of_the_linear_hold_no_tensor_memory_while_they_wait_for_their_cluster():
+    """Two kernels of clusters on two streams, each with a block that waits for the other's columns, would wait for good if blocks
+    kept theirs while they wait for their peers.  The other kernels of clusters take so much shared memory beside their columns that
+    those of one SM never run out; this one takes all columns and little more than half of the shared memory."""
+    body = dict(functions("umma_linear4.cu"))["umma_linear4_kernel"]
+    assert body.count("tcgen05.dealloc") == 1 and body.index("tcgen05.dealloc") < body.index("cluster.sync()")
+
+
 def test_codes_of_the_error_word_say_one_thing():
     """The codes that have a text of their own are no kernel's code of a wait that ran out."""
     with open(os.path.join(CSRC, "decoder.hpp")) as fh:
