@@ -427,7 +427,9 @@ class Planner {
     auto it = layout_memo_.find(key);
     if (it != layout_memo_.end()) return it->second;
     Value src = V(vi);
-    int out = add_value(src.name + (dt16 == DT::F16 ? "@f16" : "@bf16"), src.shape, dt16, src.layout);
+    std::string name = src.name + (dt16 == DT::F16 ? "@f16" : "@bf16");
+    while (S.index_.count(name)) name += "'";  // the typed value that `src` is the f32 copy of has that name
+    int out = add_value(name, src.shape, dt16, src.layout);
     V(out).bytes = src.bytes / 2;  // padded layouts (the stem's row windows) keep their padding
     const int64_t lanes = (int64_t)(src.bytes / 4);
     Step& st = add_step(n, dt16 == DT::F16 ? "convert_f32_to_f16" : "convert_f32_to_bf16", 2, {vi}, {out});

@@ -343,3 +343,17 @@ def test_a_linear_and_a_small_product_on_two_streams():
         b.enqueue(streams[1].cuda_stream)
     a.wait(), b.wait()
     assert torch.equal(y, first) and torch.equal(z, second)
+
+
+# ---- beside operators on f32 lanes -----------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+def test_a_typed_input_of_a_product_with_16_bit_weights(kind):
+    """The product takes 16-bit operands: its copy of the input's f32 lanes stands beside the input in its own type."""
+    g = torch.Generator().manual_seed(90)
+    x, w = torch.randn(24, 64, generator=g).to(D.TYPES[kind]), torch.randn(64, 32, generator=g).half()
+    graph = Graph([Node("MatMul", "m", ["x", "w"], ["y"], {}), Node("Add", "a", ["y", "b"], ["z"], {})], ["x"], ["z"])
+    got = Session.builder().with_input_types({"x": kind}).build_from_graph(graph, {"w": w.numpy(), "b": np.ones(32, np.float32)}).run({"x": x.float().numpy()})["z"]
+    want = x.double() @ w.double() + 1
+    # bf16 rows meet f16 weights as whichever type the product takes, rounded once
+    size = x.double().abs() @ w.double().abs()
+    G.within(torch.from_numpy(got), want, (2.0**-11 if kind == "bfloat16" else 0.0) * size + 66 * 2.0**-23 * (size + 1))
