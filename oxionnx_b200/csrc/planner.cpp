@@ -457,9 +457,9 @@ class Planner {
   }
 
   // Every producer decides whether to round its output to TF32 by asking this about its output's name; a "yes"
-  // is remembered, so that a contraction can tell whether its operand arrives rounded (tf32_ready).
+  // (never where a 4-bit linear or a cache takes all of the lanes' bits: a contraction then makes a rounded copy of its own) is remembered, so that a contraction can tell whether its operand arrives rounded (tf32_ready).
   bool feeds_contraction(const std::string& name) {
-    const bool yes = feeds_contraction_impl(name);
+    const bool yes = feeds_contraction_impl(name) && !feeds_typed(name);
     if (yes) tf32_rounded_names_.insert(name);
     return yes;
   }
@@ -500,6 +500,18 @@ class Planner {
     };
     layout_memo_[key] = out;
     return out;
+  }
+  // Does one of the typed operators read the value, directly or behind nodes that move or select lanes?
+  bool feeds_typed(const std::string& name) const {
+    auto it = consumers_.find(name);
+    if (it == consumers_.end()) return false;
+    static const std::set<std::string> movers = {"MaxPool", "Flatten", "Reshape", "Identity", "Relu", "Pad", "Resize", "Concat", "Transpose", "Slice", "Gather", "Cast"};
+    for (const auto& c : it->second) {
+      const NodeDef& n = nodes_[c.first];
+      if (typed_op(n.op)) return true;
+      if (movers.count(n.op) && !n.outputs.empty() && feeds_typed(n.outputs[0])) return true;
+    }
+    return false;
   }
   bool feeds_contraction_impl(const std::string& name) {
     auto it = consumers_.find(name);

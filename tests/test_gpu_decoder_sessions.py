@@ -357,3 +357,24 @@ def test_a_typed_input_of_a_product_with_16_bit_weights(kind):
     # bf16 rows meet f16 weights as whichever type the product takes, rounded once
     size = x.double().abs() @ w.double().abs()
     G.within(torch.from_numpy(got), want, (2.0**-11 if kind == "bfloat16" else 0.0) * size + 66 * 2.0**-23 * (size + 1))
+
+
+@pytest.mark.parametrize("views", [[], ["Identity"], ["Relu", "Reshape"]])
+def test_rows_that_a_product_reads_too_are_whole_to_a_linear(views):
+    """A product's output that another product reads leaves as TF32, the operands of that; a 4-bit linear that reads it too takes
+    all of its bits, the same as without the other product."""
+    g = torch.Generator().manual_seed(91)
+    w = D.linear_weights(g, 48, 64, 32, True, False)
+    x, m, o = torch.randn(40, 96, generator=g), torch.randn(96, 64, generator=g), torch.randn(64, 16, generator=g)
+    weights = {**w, "m": m.numpy(), "o": o.numpy(), "shape": np.array([40, 64], np.float32)}
+    nodes, last = [Node("MatMul", "m", ["x", "m"], ["a"], {})], "a"
+    for i, op in enumerate(views):
+        nodes.append(Node(op, f"view{i}", [last, "shape"] if op == "Reshape" else [last], [f"v{i}"], {}))
+        last = f"v{i}"
+    nodes.append(Node(*G.linear_node(64, 48, 32, w, "y", last)))
+    want = Session.builder().build_from_graph(Graph(nodes, ["x"], ["y"]), weights).run({"x": x.numpy()})["y"]
+    got = Session.builder().build_from_graph(Graph([*nodes, Node("MatMul", "o", ["a", "o"], ["p"], {})], ["x"], ["y", "p"]), weights).run({"x": x.numpy()})
+    assert np.array_equal(got["y"], want)
+    a = x.double() @ m.double()
+    size = x.double().abs() @ m.double().abs() @ o.double().abs()
+    G.within(torch.from_numpy(got["p"]), a @ o.double(), (4 * 2.0**-11 + 164 * 2.0**-23) * (1 + 2.0**-9) * size)
