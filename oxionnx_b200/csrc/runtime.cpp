@@ -572,12 +572,15 @@ void Session::stage_out(void* dst, const void* src, size_t bytes) {
 }
 
 // The context's stream is about to work on the session's memory: behind the last run that was enqueued on a caller's stream, and
-// (until the host has waited for it, sync) in front of the next one, whatever becomes of the call.  A second stream goes along.
-void Session::begin_own_work(cudaStream_t also) {
+// (until the host has waited for it, sync) in front of the next one, whatever becomes of the call.  A stream of uploads goes along.
+void Session::begin_own_work(cudaStream_t uploads) {
   own_open_ = true;
+  if (uploads && uploads_follow_) {
+    OXB_CUDA(cudaStreamWaitEvent(uploads, enqueued_ev_, 0));
+    uploads_follow_ = false;
+  }
   if (!enqueued_) return;
   OXB_CUDA(cudaStreamWaitEvent(ctx_->stream(), enqueued_ev_, 0));
-  if (also) OXB_CUDA(cudaStreamWaitEvent(also, enqueued_ev_, 0));
   enqueued_ = false;  // the context's stream stands for it
 }
 
@@ -601,7 +604,7 @@ void Session::follow_earlier_runs(cudaStream_t s) {
 void Session::end_enqueued(cudaStream_t s) {
   OXB_CUDA(cudaEventRecord(enqueued_ev_, s));
   OXB_CUDA(cudaStreamGetId(s, &enqueued_on_));
-  enqueued_ = true;
+  enqueued_ = uploads_follow_ = true;
 }
 
 static bool skipped(const Step& st, bool lanes_wanted, const std::vector<char>& typed) {

@@ -218,7 +218,8 @@ class Session {
   unsigned long long enqueued_on_ = 0;  // id of its stream
   bool enqueued_ = false;
   bool own_open_ = false;  // the context's stream may hold work of this session that nobody has waited for
-  void begin_own_work(cudaStream_t also = nullptr);
+  bool uploads_follow_ = false;  // the stream of the pipelined runs' uploads has not been put behind it yet
+  void begin_own_work(cudaStream_t uploads = nullptr);
   void follow_earlier_runs(cudaStream_t s);
   void end_enqueued(cudaStream_t s);
   void unbind_inputs();

@@ -378,3 +378,36 @@ def test_rows_that_a_product_reads_too_are_whole_to_a_linear(views):
     a = x.double() @ m.double()
     size = x.double().abs() @ m.double().abs() @ o.double().abs()
     G.within(torch.from_numpy(got["p"]), a @ o.double(), (4 * 2.0**-11 + 164 * 2.0**-23) * (1 + 2.0**-9) * size)
+
+
+def test_a_pipelined_run_uploads_behind_an_enqueued_one():
+    """An input that the product's kernel reads at a fixed address is copied there by the enqueued run, behind 100 ms of sleep, and
+    uploaded there by the pipelined one: the upload is the later of the two, also when a refused call came in between."""
+    g = torch.Generator().manual_seed(92)
+    w, x = torch.randint(-127, 128, (256, 128), generator=g), torch.randint(0, 255, (512, 256), generator=g, dtype=torch.uint8)
+    u, z = x.cuda(), torch.empty(512, 128, device="cuda")
+    graph = Graph([Node("MatMulInteger", "product", ["u", "w"], ["p"], {}), Node("Cast", "c", ["p"], ["z"], {"to": 1})], ["u"], ["z"])
+    s = Session.builder().with_input_types({"u": np.uint8}).with_input_shapes({"u": (512, 256)}).build_from_graph(graph, {"w": w.float().numpy()})
+    s.ensure_planned()
+    s.bind_input_device("u", u.data_ptr(), np.uint8, u.numel())
+    s.bind_output_device("z", z.data_ptr(), z.numel())
+    G.run(s)
+    first = z.clone()
+    assert torch.equal(first.cpu().long(), x.long() @ w)
+    feeds = {"u": (x // 2).numpy()}
+    half = s.run(feeds)["z"]
+    assert np.array_equal(half, ((x // 2).long() @ w).float().numpy())
+    assert np.array_equal(s.run_pipelined([feeds])[0]["z"], half)
+    one = torch.cuda.Stream()
+    for refused in (False, True):
+        z.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            torch.cuda._sleep(200_000_000)
+        s.enqueue(one.cuda_stream)
+        if refused:
+            assert _ffi.lib().oxb200_run(s.ctx.handle, None, 0, (_ffi.Result * 1)(), 1) == _ffi.FAILED
+        s.submit(feeds)
+        assert np.array_equal(s.collect()["z"], half)
+        one.synchronize()
+        assert torch.equal(z, first)
