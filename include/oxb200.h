@@ -187,7 +187,7 @@ typedef struct {
  *   kv_lengths, page_table.  Row i of a sequence's n new ones sees its tokens 0 .. kv_lengths - n + i; a row that sees none
  *   gets zeros.  attrs num_heads, kv_num_heads, scale (1 / sqrt(size)), max_query_length (a promise on the new tokens of a
  *   sequence, checked on the device; 0: none).  Output [.., heads * size] in the caches' type.  Results do not depend on the
- *   order in which blocks finish.  A NaN or an infinity among a sequence's later values may reach earlier rows of the same call,
+ *   order in which blocks finish, and scores may be as large as f32 holds.  A NaN or an infinity among a sequence's later values may reach earlier rows of the same call,
  *   whose probabilities for them are 0; what lies in a page behind the sequence does not. */
 
 /* oxionnx_cuda::is_supported_op (src/lib.rs:217).  Adds the INT8 family the reference's
@@ -347,9 +347,11 @@ int oxb200_bind_output_device(oxb200_ctx* ctx, const char* name, void* device_pt
  *                       launches are in the stream.  Bound buffers follow that stream's order like any kernel's operands.
  *                       Runs of one session follow one another whatever their streams; a stream that is being captured
  *                       takes the launches into its graph with the addresses bound now, and its replays are then the
- *                       caller's to order against the session's other runs.  The caller's current device is kept.
+ *                       caller's to order against the session's other runs.  The caller's current device is kept.  A call that
+ *                       fails leaves what it had launched in the order of the runs.
  *   run_wait            waits for the enqueued runs and reports what their kernels found wrong (a page table entry outside
- *                       the cache, ...), as every call that fences does. */
+ *                       the cache, ...), as every call that fences does.  It does not wait for replays of captured runs:
+ *                       let those end first, since behind an error it clears what kernels may have left half done. */
 int oxb200_bind_output_device_typed(oxb200_ctx* ctx, const char* name, void* device_ptr, int32_t dtype, uint64_t cap);
 int oxb200_run_enqueue(oxb200_ctx* ctx, void* cuda_stream);
 int oxb200_run_wait(oxb200_ctx* ctx);

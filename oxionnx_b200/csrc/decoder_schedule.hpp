@@ -2,8 +2,8 @@
 //
 // A work item is a block of 2 * `span` new tokens of one sequence for one key head (the two tiles of the kernel, `span` tokens
 // times the query heads of a key head each), over all its 128-key tiles.  All items' tiles are laid end to end, a sequence's
-// blocks in order and the key heads of a block side by side, every item with one step more for what it costs to begin and to
-// end one; a thread block takes an equal run of steps, wherever that cuts an item.
+// blocks in order and the key heads of a block side by side, every item with kBegin steps more for what it costs to begin
+// and to end one; a thread block takes an equal run of steps, wherever that cuts an item.
 #pragma once
 
 #ifndef OXB_HD

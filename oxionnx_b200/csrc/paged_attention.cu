@@ -5,9 +5,9 @@
 // its new token r / group), so that a tile of keys is read once for all of them.
 //
 // Sequences of few packed rows (single tokens of a decoding step) are bound by the bytes of their keys and values: this
-// file's kernel streams those, at 5.6 TB/s over 64 streams of up to 8100 tokens (196 us) and 5.2 over one of 131000 (103 us,
-// 10 of them beginning and joining), 32 heads on 8 key heads of 128.  Sequences of many are bound by the products and run on tcgen05 (umma_prompt.cu).  Each
-// kernel finds its own sequences in the row bounds and skips the others.
+// file's kernel streams those, at 5.5 TB/s over 64 streams of up to 8100 tokens (196 to 202 us, by the GPU) and 5.2 over one of
+// 131000 (103 us, 10 of them beginning and joining), 32 heads on 8 key heads of 128.  Sequences of many are bound by the products
+// and run on tcgen05 (umma_prompt.cu).  Each kernel finds its own sequences in the row bounds and skips the others.
 #include <algorithm>
 #include <mutex>
 

@@ -22,7 +22,7 @@
 // Every wait is bounded.
 //
 // A step (both tiles by 128 keys of 128 lanes) takes 4000 cycles, of which the products are 2048 and the exponentials as many:
-// 8192 tokens of 32 heads on 8 take 553 us, 995 TFLOP/s, at the power cap.  64 keys a step in two buffers (products of 64
+// 8192 tokens of 32 heads on 8 take 557 us, 987 TFLOP/s, at the power cap.  64 keys a step in two buffers (products of 64
 // columns run at half rate), polynomials for a part of the exponentials and a second issuing thread were no faster.
 #include <algorithm>
 #include <mutex>
